@@ -62,6 +62,39 @@ class GemmState(ctypes.Structure):
     ]
 
 
+HALF_FP16, HALF_BF16 = 0, 1
+STATUS_BAD_PAGE = 16
+
+
+class KVCache(ctypes.Structure):
+    """Mirror of ``abq_kv_cache``."""
+    _fields_ = [("data", ctypes.c_void_p), ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("bits", ctypes.c_int), ("half_type", ctypes.c_int)]
+
+
+_KV_STRIDES = [(n, ctypes.c_longlong) for n in ("k_stride", "k_head_stride", "v_stride", "v_head_stride")]
+
+
+class KVWriteParams(ctypes.Structure):
+    """Mirror of ``abq_kv_write_params``."""
+    _fields_ = [("cache", KVCache), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), *_KV_STRIDES, ("slots", ctypes.c_void_p), ("tokens", ctypes.c_int)]
+
+
+class KVReadParams(ctypes.Structure):
+    """Mirror of ``abq_kv_read_params``."""
+    _fields_ = [("cache", KVCache), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), *_KV_STRIDES, ("rows", ctypes.c_int), ("batch", ctypes.c_int),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int), ("cu_seqlens", ctypes.c_void_p)]
+
+
+class CacheAttentionParams(ctypes.Structure):
+    """Mirror of ``abq_cache_attention_params``."""
+    _fields_ = [("cache", KVCache), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                *[(n, ctypes.c_longlong) for n in ("q_stride", "q_head_stride", "out_stride", "out_head_stride")],
+                ("batch", ctypes.c_int), ("rows_per_seq", ctypes.c_int), ("q_heads", ctypes.c_int), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("seq_lens", ctypes.c_void_p), ("tree", ctypes.c_void_p), ("scale", ctypes.c_float), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t), ("status_word", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -100,6 +133,13 @@ def lib() -> ctypes.CDLL:
         L.abq_rmsnorm_quantize_pack_half.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_float] + [ctypes.c_void_p] * 4 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
         L.abq_unpack_int8.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                       ctypes.c_void_p]
+        L.abq_kv_cache_bytes.restype = ctypes.c_size_t
+        L.abq_kv_cache_bytes.argtypes = [ctypes.POINTER(KVCache)]
+        L.abq_kv_cache_write.argtypes = [ctypes.POINTER(KVWriteParams), ctypes.c_void_p]
+        L.abq_kv_cache_read.argtypes = [ctypes.POINTER(KVReadParams), ctypes.c_void_p]
+        L.abq_cache_attention_workspace_bytes.restype = ctypes.c_size_t
+        L.abq_cache_attention_workspace_bytes.argtypes = [ctypes.POINTER(KVCache), ctypes.c_int, ctypes.c_int, ctypes.c_int]
+        L.abq_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionParams), ctypes.c_void_p]
         _lib = L
     return _lib
 
@@ -278,3 +318,111 @@ def add_half(a, b, out, n: int, stream=None) -> None:
 
 def unpack_int8(planes, out_i8, rows: int, K: int, bits: int, signed: bool, stream=None) -> None:
     _check(lib().abq_unpack_int8(_ptr(planes), _ptr(out_i8), rows, K, bits, int(signed), _stream(stream)), "abq_unpack_int8")
+
+
+# ---- the quantised key/value cache and attention.  A parameter block is made once and used for many calls (it keeps its tensors alive).
+
+def _half_type(dtype) -> int:
+    import torch
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"attention takes fp16 or bf16, not {dtype}")
+    return HALF_BF16 if dtype == torch.bfloat16 else HALF_FP16
+
+
+def _rows_of(t, heads, head_dim: int, half_type: int, what: str):
+    """(address, row stride, head stride) of [rows][heads][head_dim] values, any strides that keep a head's values together."""
+    if t.dim() != 3 or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what} is {tuple(t.shape)}, expected [rows][{heads if heads is not None else 'heads'}][{head_dim}]")
+    if not t.is_cuda or _half_type(t.dtype) != half_type:
+        raise ValueError(f"{what}: a CUDA tensor of the cache's 16-bit type, not {t.dtype} on {t.device}")
+    if t.stride(2) != 1:
+        raise ValueError(f"{what}: the values of a head must lie together")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _ints(t, shape, what: str, dtype: str = "int32"):
+    import torch
+    if t.dtype != getattr(torch, dtype) or not t.is_cuda or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: a contiguous CUDA {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def kv_cache_bytes(num_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int) -> int:
+    """Bytes of one layer's cache (0: no such cache)."""
+    return int(lib().abq_kv_cache_bytes(ctypes.byref(KVCache(None, num_pages, page_size, kv_heads, head_dim, bits, HALF_FP16))))
+
+
+def make_kv_cache(data, *, page_size: int, kv_heads: int, head_dim: int, bits: int, dtype) -> KVCache:
+    """A cache of as many whole pages as ``data`` (uint8) has room for, for keys and values of ``dtype``."""
+    page = kv_cache_bytes(1, page_size, kv_heads, head_dim, bits)
+    pages = data.numel() * data.element_size() // page if page else 0
+    if not pages:
+        raise ValueError(f"no cache of {bits} bits, {kv_heads} heads of {head_dim}, pages of {page_size} tokens in {data.numel() * data.element_size()} bytes")
+    c = KVCache(_ptr(data), pages, page_size, kv_heads, head_dim, bits, _half_type(dtype))
+    c._keep_alive = data
+    return c
+
+
+def make_kv_write_params(cache: KVCache, k, v, slots) -> KVWriteParams:
+    """k, v [tokens][kv_heads][head_dim] (views with strides are fine), slots int64 [tokens]: page * page_size + place, negative = left out."""
+    p = KVWriteParams()
+    p.cache, p.tokens = cache, k.shape[0]
+    p.k, p.k_stride, p.k_head_stride = _rows_of(k, cache.kv_heads, cache.head_dim, cache.half_type, "k")
+    p.v, p.v_stride, p.v_head_stride = _rows_of(v, cache.kv_heads, cache.head_dim, cache.half_type, "v")
+    if v.shape[0] != p.tokens:
+        raise ValueError(f"{p.tokens} rows of k, {v.shape[0]} of v")
+    p.slots = _ints(slots, (p.tokens,), "slots", "int64")
+    p._keep_alive = (cache, k, v, slots)
+    return p
+
+
+def kv_cache_write(params: KVWriteParams, stream=None) -> None:
+    _check(lib().abq_kv_cache_write(ctypes.byref(params), _stream(stream)), "abq_kv_cache_write")
+
+
+def make_kv_read_params(cache: KVCache, k, v, block_table, cu_seqlens) -> KVReadParams:
+    """k, v [rows][kv_heads][head_dim] get the sequences packed; block_table int32 [batch][pages], cu_seqlens int32 [batch + 1]."""
+    p = KVReadParams()
+    p.cache, p.rows = cache, k.shape[0]
+    p.k, p.k_stride, p.k_head_stride = _rows_of(k, cache.kv_heads, cache.head_dim, cache.half_type, "k")
+    p.v, p.v_stride, p.v_head_stride = _rows_of(v, cache.kv_heads, cache.head_dim, cache.half_type, "v")
+    if v.shape[0] != p.rows:
+        raise ValueError(f"{p.rows} rows of k, {v.shape[0]} of v")
+    p.batch, p.table_stride = block_table.shape
+    p.block_table = _ints(block_table, (p.batch, p.table_stride), "block_table")
+    p.cu_seqlens = _ints(cu_seqlens, (p.batch + 1,), "cu_seqlens")
+    p._keep_alive = (cache, k, v, block_table, cu_seqlens)
+    return p
+
+
+def kv_cache_read(params: KVReadParams, stream=None) -> None:
+    _check(lib().abq_kv_cache_read(ctypes.byref(params), _stream(stream)), "abq_kv_cache_read")
+
+
+def cache_attention_workspace_bytes(cache: KVCache, batch: int, rows_per_seq: int, q_heads: int) -> int:
+    return int(lib().abq_cache_attention_workspace_bytes(ctypes.byref(cache), batch, rows_per_seq, q_heads))
+
+
+def make_cache_attention_params(cache: KVCache, q, out, block_table, seq_lens, *, scale: float, workspace, tree=None, status_word=None) -> CacheAttentionParams:
+    """q, out [batch * n][q_heads][head_dim]: the last n tokens of every sequence; block_table int32 [batch][pages], seq_lens int32 [batch]
+    (those tokens included), tree int64 [batch][n]: bit j of a row = it sees draft j (None: each sees those up to itself)."""
+    p = CacheAttentionParams()
+    p.cache = cache
+    p.batch, p.table_stride = block_table.shape
+    if q.dim() != 3 or out.shape != q.shape or (q.shape[0] % p.batch if p.batch else q.shape[0]):
+        raise ValueError(f"q {tuple(q.shape)} and out {tuple(out.shape)} do not hold the same rows of {p.batch} sequences")
+    p.rows_per_seq, p.q_heads = q.shape[0] // p.batch if p.batch else 1, q.shape[1]
+    p.q, p.q_stride, p.q_head_stride = _rows_of(q, None, cache.head_dim, cache.half_type, "q")
+    p.out, p.out_stride, p.out_head_stride = _rows_of(out, None, cache.head_dim, cache.half_type, "out")
+    p.block_table = _ints(block_table, (p.batch, p.table_stride), "block_table")
+    p.seq_lens = _ints(seq_lens, (p.batch,), "seq_lens")
+    p.tree = None if tree is None else _ints(tree, (p.batch, p.rows_per_seq), "tree", "int64")
+    p.scale = scale
+    p.workspace, p.workspace_bytes = _ptr(workspace), workspace.numel() * workspace.element_size()
+    p.status_word = _ptr(status_word)
+    p._keep_alive = (cache, q, out, block_table, seq_lens, tree, workspace, status_word)
+    return p
+
+
+def cache_attention(params: CacheAttentionParams, stream=None) -> None:
+    _check(lib().abq_cache_attention(ctypes.byref(params), _stream(stream)), "abq_cache_attention")

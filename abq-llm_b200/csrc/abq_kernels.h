@@ -111,6 +111,11 @@ enum TmapDtype { TMAP_U8 = 0, TMAP_U32 = 1 };
 bool encode_tmap(void *out128, TmapDtype dtype, int rank, const void *base, const uint64_t *dims, const uint64_t *strides_bytes,
                  const uint32_t *box, TmapSwizzle swizzle);
 void set_last_cuda_error(cudaError_t e);
+
+// ---- kv_cache.cu
+bool kv_cache_valid(const abq_kv_cache &c);
+// rows of 16-bit values that are moved 16 bytes at a time: pointer and strides (in elements)
+bool half_rows_valid(const void *p, long long stride, long long head_stride);
 int env_int(const char *name, int fallback);
 
 } // namespace abq

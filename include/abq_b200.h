@@ -345,6 +345,100 @@ ABQ_API abq_status abq_unpack_int8(const void *planes, void *out_i8, int rows, i
 #define ABQ_STATIC_SCRATCH_BYTES (16u << 20)
 ABQ_API abq_status abq_gemm_static_scratch(const abq_gemm_params *params, abq_stream_t stream);
 
+/*
+ * Attention over a quantised key/value cache, and over whole prompts: the step between the QKV projection and the attention output
+ * projection of a decoder block.  (The reference's FasterTransformer fork runs its fp16 attention there, layers/attention_layers/
+ * {GptContextAttentionLayer,DecoderSelfAttentionLayer}.cc; it has no quantised cache, no trees of drafted tokens and no packed
+ * prompts.)  Queries, keys, values and results are fp16 or bf16; heads are 64 or 128 wide; q_heads is a multiple of kv_heads (head h of the
+ * queries reads head h / (q_heads / kv_heads) of the cache).  Strides count elements; every pointer is 16-byte aligned and every stride a
+ * multiple of 8, so slices of a fused QKV buffer are fine.  All four calls join a programmatic-dependent-launch chain: they read and write
+ * after waiting for the kernel ahead of them.
+ */
+typedef enum abq_half_type { ABQ_HALF_FP16 = 0, ABQ_HALF_BF16 = 1 } abq_half_type;
+
+/*
+ * One layer's paged cache (caller-owned memory, plain data).  data: [num_pages][kv_heads][page_size / 16][granule], a granule being 16
+ * tokens of one head: 16 rows of key codes, 16 rows of value codes, 16 pairs (scale, min) of the keys, 16 of the values in the 16-bit type.
+ * A row is head_dim * bits / 8 bytes, codes in order (4 bits: the even one in the low nibble), value = min + code * scale.  Inside the
+ * 16 rows, 16-byte piece p of 128-byte line l lies at piece p ^ x(l): x = 2 (l % 4) ^ 4 (l / 4 % 2) for rows of 128 bytes, 2 (l % 4) for
+ * rows of 64, 4 (l % 2) for rows of 32 (the order that the attention kernel reads without bank conflicts).
+ * Token position t of a sequence lies in the page its block table names for t / page_size, at place t % page_size.
+ */
+typedef struct abq_kv_cache {
+    void *data;      /* abq_kv_cache_bytes() bytes, 16-byte aligned */
+    int num_pages;
+    int page_size;   /* tokens: a multiple of 16, at most 1024 */
+    int kv_heads;
+    int head_dim;    /* 64 or 128 */
+    int bits;        /* 8 or 4 */
+    int half_type;   /* abq_half_type of what is written to it and read from it */
+} abq_kv_cache;
+
+/* Bytes of the cache's data; 0 for a description that is not valid (data itself is not looked at). */
+ABQ_API size_t abq_kv_cache_bytes(const abq_kv_cache *cache);
+
+/*
+ * Quantise the keys and values of `tokens` rows and write them to their places.  Per token and head, min/max calibration as the reference's
+ * dynamic quantiser has it (algorithm/quantize/quantizer.py:149-179), in fp32: scale = (max - min) / (2^bits - 1) rounded up to the 16-bit
+ * type, code = rint((x - min) / scale); min is an input value and kept as it is.  A row whose max - min is not finite (Inf, NaN) is stored as
+ * scale = min = NaN: it reads as NaN.
+ *   slots   device int64 [tokens]: page * page_size + place; rows whose slot is negative or outside the cache are left out (padding).
+ *           The slots of one call are distinct: two rows for one place may leave a mixture of both there.
+ */
+typedef struct abq_kv_write_params {
+    abq_kv_cache cache;
+    const void *k, *v; /* [tokens][kv_heads][head_dim] */
+    long long k_stride, k_head_stride, v_stride, v_head_stride;
+    const int64_t *slots;
+    int tokens;
+} abq_kv_write_params;
+ABQ_API abq_status abq_kv_cache_write(const abq_kv_write_params *params, abq_stream_t stream);
+
+/*
+ * Read whole sequences back, packed: row cu_seqlens[b] + t of k and v gets position t of sequence b.  Feeds abq_prompt_attention with the
+ * prefix of a chunk.  Rows from cu_seqlens[batch] on are left as they were; positions whose page is outside the table's row or the cache give 0.
+ */
+typedef struct abq_kv_read_params {
+    abq_kv_cache cache;
+    void *k, *v; /* [rows][kv_heads][head_dim] */
+    long long k_stride, k_head_stride, v_stride, v_head_stride;
+    int rows;               /* rows that k and v have room for: later ones are not written */
+    int batch;
+    const int *block_table; /* device int32 [batch][table_stride]: pages */
+    int table_stride;
+    const int *cu_seqlens;  /* device int32 [batch + 1], starting at 0, never falling */
+} abq_kv_read_params;
+ABQ_API abq_status abq_kv_cache_read(const abq_kv_read_params *params, abq_stream_t stream);
+
+/*
+ * Attention of the last rows_per_seq (n <= 64) tokens of every sequence over its cached keys and values, theirs included: one token of a decode step
+ * (n = 1), or a tree of drafted tokens that are verified at once.  Sequence b holds seq_lens[b] tokens; token seq_lens[b] - n + j is draft j.
+ * Row i sees every token before the drafts, and draft j where bit j of tree[b][i] is set (without `tree`: j <= i).  A row that sees no
+ * token gives 0 (a sequence of length 0 among them).  out = sum_j softmax_j(scale * q . k_j) v_j in fp32; products run on the tensor cores in
+ * fp16, on codes that fp16 holds exactly.
+ * Lengths are read on the device (a captured launch follows them); they are bounded by table_stride * page_size.  Pages outside the
+ * cache are not read: their tokens count as unseen and ABQ_STATUS_BAD_PAGE is set in the status word, if there is one.
+ * The workspace is scratch of this call alone: calls that may overlap need one each.
+ */
+#define ABQ_STATUS_BAD_PAGE 16
+typedef struct abq_cache_attention_params {
+    abq_kv_cache cache;
+    const void *q; /* [batch * rows_per_seq][q_heads][head_dim] */
+    void *out;     /* the same shape; may be q itself */
+    long long q_stride, q_head_stride, out_stride, out_head_stride;
+    int batch, rows_per_seq, q_heads;
+    const int *block_table; /* device int32 [batch][table_stride]: pages */
+    int table_stride;
+    const int *seq_lens;    /* device int32 [batch] */
+    const uint64_t *tree;   /* optional device [batch][rows_per_seq] */
+    float scale;
+    void *workspace;        /* abq_cache_attention_workspace_bytes(), 16-byte aligned */
+    size_t workspace_bytes;
+    int *status_word;       /* optional */
+} abq_cache_attention_params;
+ABQ_API size_t abq_cache_attention_workspace_bytes(const abq_kv_cache *cache, int batch, int rows_per_seq, int q_heads);
+ABQ_API abq_status abq_cache_attention(const abq_cache_attention_params *params, abq_stream_t stream);
+
 /* Text for a status code; cudaError_t of the last failing CUDA call in this thread (0 if none). */
 ABQ_API const char *abq_status_string(abq_status s);
 ABQ_API int abq_last_cuda_error(void);
