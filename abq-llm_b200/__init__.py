@@ -12,5 +12,6 @@ from .binding import (  # noqa: F401
     HALF_FP16, HALF_BF16, STATUS_BAD_PAGE, KVCache, KVWriteParams, KVReadParams, CacheAttentionParams,
     kv_cache_bytes, make_kv_cache, make_kv_write_params, kv_cache_write, make_kv_read_params, kv_cache_read,
     cache_attention_workspace_bytes, make_cache_attention_params, cache_attention,
+    PromptAttentionParams, make_prompt_attention_params, prompt_attention,
 )
 from .wrapper import ABQGEMMWrapper, launch_pack, launch_pack4  # noqa: F401

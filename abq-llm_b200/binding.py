@@ -95,6 +95,15 @@ class CacheAttentionParams(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t), ("status_word", ctypes.c_void_p)]
 
 
+class PromptAttentionParams(ctypes.Structure):
+    """Mirror of ``abq_prompt_attention_params``."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                *[(n + s, ctypes.c_longlong) for n in ("q", "k", "v", "out") for s in ("_stride", "_head_stride")],
+                ("total_q", ctypes.c_int), ("total_k", ctypes.c_int), ("q_heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("half_type", ctypes.c_int), ("batch", ctypes.c_int), ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p), ("max_q", ctypes.c_int),
+                ("scale", ctypes.c_float), ("status_word", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -140,6 +149,7 @@ def lib() -> ctypes.CDLL:
         L.abq_cache_attention_workspace_bytes.restype = ctypes.c_size_t
         L.abq_cache_attention_workspace_bytes.argtypes = [ctypes.POINTER(KVCache), ctypes.c_int, ctypes.c_int, ctypes.c_int]
         L.abq_cache_attention.argtypes = [ctypes.POINTER(CacheAttentionParams), ctypes.c_void_p]
+        L.abq_prompt_attention.argtypes = [ctypes.POINTER(PromptAttentionParams), ctypes.c_void_p]
         _lib = L
     return _lib
 
@@ -426,3 +436,26 @@ def make_cache_attention_params(cache: KVCache, q, out, block_table, seq_lens, *
 
 def cache_attention(params: CacheAttentionParams, stream=None) -> None:
     _check(lib().abq_cache_attention(ctypes.byref(params), _stream(stream)), "abq_cache_attention")
+
+
+def make_prompt_attention_params(q, k, v, out, cu_q, cu_k, *, scale: float, max_q: int = 0, status_word=None) -> PromptAttentionParams:
+    """q, out [total_q][q_heads][head_dim], k, v [total_k][kv_heads][head_dim] (views with strides are fine) of sequences packed behind one another;
+    cu_q, cu_k int32 [batch + 1]: where each starts.  ``max_q``: rows of the longest, where known."""
+    p = PromptAttentionParams()
+    if q.dim() != 3 or k.dim() != 3 or out.shape != q.shape or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and out {tuple(out.shape)} do not belong together")
+    p.total_q, p.q_heads, p.head_dim = q.shape
+    p.total_k, p.kv_heads = k.shape[:2]
+    p.half_type = _half_type(q.dtype)
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        at, rows, heads = _rows_of(t, None, p.head_dim, p.half_type, name)
+        setattr(p, name, at), setattr(p, name + "_stride", rows), setattr(p, name + "_head_stride", heads)
+    p.batch = cu_q.numel() - 1
+    p.cu_q, p.cu_k = _ints(cu_q, (p.batch + 1,), "cu_q"), _ints(cu_k, (p.batch + 1,), "cu_k")
+    p.scale, p.max_q, p.status_word = scale, max_q, _ptr(status_word)
+    p._keep_alive = (q, k, v, out, cu_q, cu_k, status_word)
+    return p
+
+
+def prompt_attention(params: PromptAttentionParams, stream=None) -> None:
+    _check(lib().abq_prompt_attention(ctypes.byref(params), _stream(stream)), "abq_prompt_attention")

@@ -1,0 +1,686 @@
+// Causal attention of packed prompts (abq_prompt_attention) on the fifth-generation tensor cores.
+//
+// Per block of 256 query rows of one key head: S = Q K^T over 128 keys at a time, p = 2^(scale log2(e) s - m) with the running row maximum m,
+// O = O 2^(m_old - m) + P V, at the end O / sum(p).  Operands never leave the chip between the two products: S and O are TMEM accumulators, P replaces S
+// in TMEM as the first operand of the second product, K and V tiles come by TMA.
+//
+// A row of a block is a (token, query head) pair: the largest power of two of heads that share a key head lie behind one another in a tile (TMA
+// gathers them as a box), so that short prompts fill tiles and the heads of a group share the K and V tiles.
+//
+// Roles of a CTA (one per SM, persistent over blocks, the longest of a sequence first and dealt to and fro so that long and short ones add up):
+//   warps 0-3, 4-7  softmax of the two 128-row tiles, a thread per row; they also scale O (only when the maximum has grown by more than 2^8: the
+//                   exponent stays bounded without it) and write the result
+//   warp 8          TMA: Q of a block, K and V tiles in the order of their use through one ring
+//   warp 9          issues the products: while one tile's softmax runs, the tensor cores work for the other
+//   warps 10, 11    look through the V tiles that some row of the block does not see to the end: 0 times Inf or NaN is no 0, so such values are set to 0 in
+//                   shared memory and added by the rows that see them when they write their result
+// What bounds it: the tensor cores (4 * 128 * 128 * D operations a tile pair) and, as long for D = 128 and twice as long for D = 64, one exponential per score.
+//
+// P is rounded to the 16-bit type (tensor-core operands); fp16 holds p times 2^6, so that weights down to 2^-20 of the maximum keep all bits.  The sum of p is
+// that of the unrounded values.
+#include <cuda.h>
+#include <algorithm>
+
+#include "abq_kernels.h"
+#include "kv_cache.cuh"
+#include "umma.cuh"
+
+namespace abq {
+
+constexpr int kPaThreads = 384;
+constexpr int kPaKeys = 128; // keys of a tile
+
+struct PaArgs {
+    const int *cu_q, *cu_k;
+    const uint8_t *v;
+    uint8_t *out;
+    long long v_stride, v_head_stride, out_stride, out_head_stride; // bytes
+    int total_q, total_k, batch, head_groups, pack_log2, group;
+    float scale_log2;
+    int *status;
+};
+
+template <int D>
+struct PaShape {
+    static constexpr int kTile = 128 * D * 2, kHalf = 128 * 128, kHalves = D / 64; // a 128-byte-swizzled half holds 64 features
+    static constexpr int kStages = D == 128 ? 5 : 10;
+    static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 512;
+    static constexpr int kO = 256; // TMEM columns: S / P of the tiles at 0 and 128, their O from here
+};
+
+struct PaItem {
+    int q0, nq, k0, nk, off; // rows of q and of k, keys that a row sees beyond its own index
+    int tok0, hg;            // first token of the block, group of heads
+    int n[2], most, edge;    // key tiles per row tile, the larger, the first that some row does not see to its end
+    bool valid;
+};
+
+// Block number `idx`, found by all lanes of a warp: 32 sequences at a time.
+__device__ __forceinline__ PaItem pa_item(const PaArgs &a, int idx, int lane)
+{
+    PaItem it;
+    int slot = idx / a.head_groups;
+    it.hg = idx - slot * a.head_groups;
+    it.valid = false;
+    const int tokens = 256 >> a.pack_log2;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int b = b0 + lane;
+        int q0 = 0, nq = 0, k0 = 0, nk = 0;
+        if (b < a.batch) {
+            q0 = min(max(a.cu_q[b], 0), a.total_q);
+            nq = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
+            k0 = min(max(a.cu_k[b], 0), a.total_k);
+            nk = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
+        }
+        const int blocks = (nq + tokens - 1) / tokens;
+        int end = blocks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, end, o);
+            end += lane >= o ? x : 0;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, slot < end);
+        if (behind) {
+            const int at = __ffs(behind) - 1;
+            it.q0 = __shfl_sync(0xffffffffu, q0, at);
+            it.nq = __shfl_sync(0xffffffffu, nq, at);
+            it.k0 = __shfl_sync(0xffffffffu, k0, at);
+            it.nk = __shfl_sync(0xffffffffu, nk, at);
+            it.tok0 = (__shfl_sync(0xffffffffu, end, at) - 1 - slot) * tokens; // the last block, which sees most, first
+            it.off = it.nk - it.nq;
+            it.valid = true;
+            break;
+        }
+        slot -= __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (!it.valid)
+        return it;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = it.tok0 + t * (tokens >> 1), last = min(it.nq, first + (tokens >> 1)) - 1;
+        it.n[t] = first >= it.nq ? 0 : (max(0, min(it.nk, last + it.off + 1)) + kPaKeys - 1) / kPaKeys;
+    }
+    it.most = max(it.n[0], it.n[1]);
+    it.edge = max(0, min(it.nk, it.tok0 + it.off + 1)) / kPaKeys;
+    return it;
+}
+
+// Place of a tile in the ring, counted from the block's first: K0, K1, V0, K2, V1, .. , V(n - 1)
+__device__ __forceinline__ int pa_k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int pa_v_place(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
+
+__device__ __forceinline__ float pa_ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pa_pack(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void pa_unpack(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+#define PA_REGS32(v)                                                                                                                                       \
+    "+f"((v)[0]), "+f"((v)[1]), "+f"((v)[2]), "+f"((v)[3]), "+f"((v)[4]), "+f"((v)[5]), "+f"((v)[6]), "+f"((v)[7]), "+f"((v)[8]), "+f"((v)[9]),           \
+        "+f"((v)[10]), "+f"((v)[11]), "+f"((v)[12]), "+f"((v)[13]), "+f"((v)[14]), "+f"((v)[15]), "+f"((v)[16]), "+f"((v)[17]), "+f"((v)[18]),             \
+        "+f"((v)[19]), "+f"((v)[20]), "+f"((v)[21]), "+f"((v)[22]), "+f"((v)[23]), "+f"((v)[24]), "+f"((v)[25]), "+f"((v)[26]), "+f"((v)[27]),             \
+        "+f"((v)[28]), "+f"((v)[29]), "+f"((v)[30]), "+f"((v)[31])
+
+// 32 accumulator columns of this thread's TMEM lane; the values may be used after pa_ld_wait() on them
+__device__ __forceinline__ void pa_ld32(uint32_t taddr, float *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
+                   "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
+                   "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void pa_ld_wait(float *v) { asm volatile("tcgen05.wait::ld.sync.aligned;" : PA_REGS32(v)::"memory"); }
+__device__ __forceinline__ void pa_ld_tie(float *v) { asm volatile("" : PA_REGS32(v)); } // (waited for with others)
+__device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+                 "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kPaThreads, 1)
+prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                        const __grid_constant__ PaArgs a)
+{
+    using Sh = PaShape<D>;
+    constexpr int kStages = Sh::kStages, kTile = Sh::kTile, kHalf = Sh::kHalf, kHalves = Sh::kHalves;
+    constexpr uint32_t kType = BF16 ? 1u : 0u;
+    constexpr uint32_t kIdescS = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(kPaKeys >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t kIdescO = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t *sq = smem, *ring = smem + 2 * kTile;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + kStages * kTile);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_ready = bars + 4, *drain = bars + 6;
+    uint64_t *kv_full = bars + 8, *kv_empty = kv_full + kStages, *edge_full = kv_empty + kStages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(edge_full + kStages);
+    int *poison = reinterpret_cast<int *>(tmem_slot + 2); // [2 warps][4 blocks]: V tiles of the block held Inf or NaN
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(drain, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_ready[t], 4);
+        }
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&kv_full[s], 2); // the producer twice, or the two warps that looked through the tile
+            mbar_init(&kv_empty[s], 1);
+            mbar_init(&edge_full[s], 1);
+        }
+        fence_mbar_init();
+        prefetch_tmap(&tmap_q);
+        prefetch_tmap(&tmap_k);
+        prefetch_tmap(&tmap_v);
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+
+    // The pool is what the block was launched with: 384 threads x 168 registers = 256 x 208 + 128 x 88
+    const int G = gridDim.x, c = blockIdx.x;
+    auto number = [&](int round) { return round * G + (round & 1 ? G - 1 - c : c); };
+
+    if (warp >= 8)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < 8) {
+        // ---------------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + (uint32_t)(t * 128), to = tmem + lanes + (uint32_t)(Sh::kO + t * D);
+        const int pack = 1 << a.pack_log2;
+        uint32_t phase = 0;
+        int blocks = 0; // with a key
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            const PaItem it = pa_item(a, number(round), lane);
+            if (!it.valid)
+                break;
+            const int token = it.tok0 + t * (128 >> a.pack_log2) + (row >> a.pack_log2), head = it.hg * pack + (row & (pack - 1));
+            const int sees = min(it.nk, token + it.off + 1);
+            float m = -INFINITY;
+            uint64_t sum2 = 0;
+            float l = 0.f;
+            const int n = t ? it.n[1] : it.n[0];
+            for (int j = 0; j < n; ++j) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[t], phase & 1, a.status, STATUS_TIMEOUT_MMA));
+                if (!ok)
+                    break;
+                ++phase;
+                tmem_fence_after();
+                float s[128];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    pa_ld32(ts + 32 * x, s + 32 * x);
+                pa_ld_wait(s);
+                pa_ld_tie(s + 32);
+                pa_ld_tie(s + 64);
+                pa_ld_tie(s + 96);
+                const int lim = sees - j * kPaKeys;
+                if (__any_sync(0xffffffffu, lim < kPaKeys)) {
+#pragma unroll
+                    for (int x = 0; x < 128; ++x)
+                        s[x] = x < lim ? s[x] : -INFINITY;
+                }
+                float top[4] = { s[0], s[1], s[2], s[3] };
+#pragma unroll
+                for (int x = 4; x < 128; x += 8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        top[e] = x + 4 + e < 128 ? pa_max3(top[e], s[x + e], s[x + 4 + e]) : fmaxf(top[e], s[x + e]);
+                }
+                const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                const bool raise = peak > m + 8.f;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float f = raise ? pa_ex2(m - peak) : 1.f;
+                    m = raise ? peak : m;
+                    float lo, hi;
+                    pa_unpack(sum2, lo, hi);
+                    l = (l + lo + hi) * f;
+                    sum2 = 0;
+                    if (j > 0) { // (the first product of a block overwrites O)
+#pragma unroll 1
+                        for (int x = 0; x < D; x += 32) {
+                            float o[32];
+                            pa_ld32(to + x, o);
+                            pa_ld_wait(o);
+                            uint32_t w[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                w[e] = __float_as_uint(o[e] * f);
+                            pa_st16(to + x, w);
+                            pa_st16(to + x + 16, w + 16);
+                        }
+                    }
+                }
+                const float base = (BF16 ? 0.f : 6.f) - (m == -INFINITY ? 0.f : m);
+                const uint64_t scale2 = pa_pack(a.scale_log2, a.scale_log2), base2 = pa_pack(base, base);
+#pragma unroll
+                for (int x = 0; x < 128; x += 32) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float lo, hi;
+                        pa_unpack(pa_fma2(pa_pack(s[x + e], s[x + e + 1]), scale2, base2), lo, hi);
+                        lo = pa_ex2(lo);
+                        hi = pa_ex2(hi);
+                        sum2 = pa_add2(sum2, pa_pack(lo, hi));
+                        w[e >> 1] = float_pair_to_half(lo, hi, BF16);
+                    }
+                    pa_st16(ts + (x >> 1), w);
+                }
+                pa_st_wait();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&p_ready[t]);
+            }
+            if (!ok)
+                break;
+            float inv = 0.f;
+            bool foul = false;
+            if (n > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[t], phase & 1, a.status, STATUS_TIMEOUT_MMA));
+                if (!ok)
+                    break;
+                ++phase;
+                tmem_fence_after();
+                float lo, hi;
+                pa_unpack(sum2, lo, hi);
+                l += lo + hi;
+                inv = l == 0.f ? 0.f : 1.f / l;
+                if (it.edge < it.most)
+                    foul = *reinterpret_cast<volatile int *>(&poison[blocks & 3]) | *reinterpret_cast<volatile int *>(&poison[4 + (blocks & 3)]);
+            }
+            blocks += it.most > 0;
+            uint8_t *dst = a.out + (long long)(it.q0 + token) * a.out_stride + (long long)head * a.out_head_stride;
+            const int kv_head = (it.hg << a.pack_log2) / a.group;
+#pragma unroll 1
+            for (int x = 0; x < D; x += 32) {
+                float o[32];
+                if (n > 0) {
+                    pa_ld32(to + x, o);
+                    pa_ld_wait(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        o[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    o[e] = l == 0.f ? 0.f : o[e] * inv;
+                if (foul) { // Inf and NaN among the values that this row sees in the last tiles (they were left out of the product)
+                    for (int k = it.edge * kPaKeys; k < sees; ++k) {
+                        const unsigned short *vr = reinterpret_cast<const unsigned short *>(a.v + (long long)(it.k0 + k) * a.v_stride + (long long)kv_head * a.v_head_stride) + x;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float f = half_bits_to_float(vr[e], BF16);
+                            if (!(fabsf(f) <= 3.402823466e38f))
+                                o[e] += f;
+                        }
+                    }
+                }
+                if (token < it.nq) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4 *>(dst + 2 * (x + e)) =
+                            make_uint4(float_pair_to_half(o[e], o[e + 1], BF16), float_pair_to_half(o[e + 2], o[e + 3], BF16),
+                                       float_pair_to_half(o[e + 4], o[e + 5], BF16), float_pair_to_half(o[e + 6], o[e + 7], BF16));
+                }
+            }
+            tmem_fence_before(); // (O is read before the next block's first product, which waits for this tile's p)
+        }
+    } else if (warp == 8) {
+        // ---------------------------------------------------------------- copies
+        int place = 0, blocks = 0, asked = 0, queries = 0; // tiles and blocks of queries asked for
+        uint32_t edges = 0, last_edge = 0;                 // a bit per stage: parity of edge_full; whether the last tile went there
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            const PaItem it = pa_item(a, number(round), lane);
+            if (!it.valid)
+                break;
+            if (it.most == 0)
+                continue;
+            const int pack = 1 << a.pack_log2, kv_head = (it.hg << a.pack_log2) / a.group, total = 2 * it.most;
+            bool fine = true, leader = false;
+            if (elect_one()) {
+                leader = true;
+                for (int i = 0; i < total; ++i) {
+                    if (i == 1) { // Q behind the first K tile: its place is free when the last block's S are done
+                        if (blocks && !mbar_wait_bounded(q_empty, (blocks - 1) & 1, a.status, STATUS_TIMEOUT_PIPE)) {
+                            fine = false;
+                            break;
+                        }
+                        mbar_arrive_expect_tx(q_full, (uint32_t)kTile * ((it.n[0] > 0) + (it.n[1] > 0)));
+                        ++queries;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            if (it.n[t] > 0)
+                                for (int h = 0; h < kHalves; ++h)
+                                    tma_load_3d(sq + t * kTile + h * kHalf, &tmap_q, h * 128, it.hg * pack, it.q0 + it.tok0 + t * (128 >> a.pack_log2), q_full);
+                    }
+                    const int at = place + i, s = at % kStages;
+                    if (at >= kStages && !mbar_wait_bounded(&kv_empty[s], ((at / kStages) - 1) & 1, a.status, STATUS_TIMEOUT_PIPE)) {
+                        fine = false;
+                        break;
+                    }
+                    const bool value = i == total - 1 || (i > 0 && (i & 1) == 0);
+                    const int j = i == total - 1 ? it.most - 1 : value ? (i - 2) / 2 : (i + 1) / 2;
+                    uint64_t *bar = &kv_full[s];
+                    last_edge &= ~(1u << s);
+                    if (value && j >= it.edge) {
+                        bar = &edge_full[s];
+                        edges ^= 1u << s;
+                        last_edge |= 1u << s;
+                    } else {
+                        mbar_arrive(bar);
+                    }
+                    mbar_arrive_expect_tx(bar, kTile);
+                    asked = at + 1;
+                    for (int h = 0; h < kHalves; ++h)
+                        tma_load_3d(ring + s * kTile + h * kHalf, value ? &tmap_v : &tmap_k, h * 128, kv_head, it.k0 + j * kPaKeys, bar);
+                }
+            }
+            __syncwarp();
+            const int from = __ffs(__ballot_sync(0xffffffffu, leader)) - 1;
+            ok = __shfl_sync(0xffffffffu, (int)fine, from);
+            asked = __shfl_sync(0xffffffffu, asked, from);
+            queries = __shfl_sync(0xffffffffu, queries, from);
+            edges = __shfl_sync(0xffffffffu, edges, from);
+            last_edge = __shfl_sync(0xffffffffu, last_edge, from);
+            place += total;
+            ++blocks;
+        }
+        if (!ok) { // a wait ran out: what has been asked for arrives before the block ends, whether or not it is used
+            for (int at = max(0, asked - kStages); at < asked; ++at) {
+                const int s = at % kStages;
+                if (last_edge >> s & 1)
+                    mbar_wait_bounded(&edge_full[s], (edges >> s & 1) ^ 1, a.status, STATUS_TIMEOUT_TMA);
+                else
+                    mbar_wait_bounded(&kv_full[s], (at / kStages) & 1, a.status, STATUS_TIMEOUT_TMA);
+            }
+            if (queries)
+                mbar_wait_bounded(q_full, (queries - 1) & 1, a.status, STATUS_TIMEOUT_TMA);
+        }
+    } else if (warp == 9) {
+        // ---------------------------------------------------------------- products
+        int place = 0, blocks = 0;
+        uint32_t p_phase[2] = { 0, 0 };
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            const PaItem it = pa_item(a, number(round), lane);
+            if (!it.valid)
+                break;
+            if (it.most == 0)
+                continue;
+            bool fine = true;
+            if (elect_one()) {
+                auto wait_kv = [&](int at) { return mbar_wait_bounded(&kv_full[at % kStages], (at / kStages) & 1, a.status, STATUS_TIMEOUT_TMA); };
+                auto scores = [&](int t, int at) {
+                    const uint32_t qa = smem_u32(sq + t * kTile), ka = smem_u32(ring + (at % kStages) * kTile);
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) {
+                        const uint64_t dq = make_smem_desc_sw128(qa + h * kHalf), dk = make_smem_desc_sw128(ka + h * kHalf);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) // 16 features of 2 bytes a step
+                            umma_f16(tmem + (uint32_t)(t * 128), dq + (uint64_t)(2 * x), dk + (uint64_t)(2 * x), kIdescS, (h | x) != 0);
+                    }
+                    umma_commit(&s_full[t]);
+                };
+                fine = mbar_wait_bounded(q_full, blocks & 1, a.status, STATUS_TIMEOUT_TMA) && wait_kv(place);
+                if (fine) {
+                    tmem_fence_after();
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (it.n[t] > 0)
+                            scores(t, place);
+                    umma_commit(&kv_empty[place % kStages]);
+                    if (it.most == 1)
+                        umma_commit(q_empty);
+                }
+                for (int j = 0; j < it.most && fine; ++j) {
+                    const int vat = place + pa_v_place(j, it.most), kat = place + pa_k_place(j + 1);
+                    bool have_v = false, have_k = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= it.n[t] || !fine)
+                            continue;
+                        fine = mbar_wait_bounded(&p_ready[t], (p_phase[t] + j) & 1, a.status, STATUS_TIMEOUT_PIPE) && (have_v || wait_kv(vat));
+                        if (!fine)
+                            continue;
+                        have_v = true;
+                        tmem_fence_after();
+                        const uint64_t dv = make_smem_desc_sw128_mn(smem_u32(ring + (vat % kStages) * kTile), kHalf);
+#pragma unroll
+                        for (int x = 0; x < kPaKeys / 16; ++x) // 16 keys a step: 16 rows of V, 8 columns of P
+                            umma_f16_ts(tmem + (uint32_t)(Sh::kO + t * D), tmem + (uint32_t)(t * 128 + 8 * x), dv + (uint64_t)(x * 2048 >> 4), kIdescO, (j | x) != 0);
+                        if (j == it.n[t] - 1) {
+                            umma_commit(&s_full[t]); // O is complete
+                        } else {
+                            fine = have_k || wait_kv(kat);
+                            if (!fine)
+                                continue;
+                            have_k = true;
+                            tmem_fence_after();
+                            scores(t, kat);
+                        }
+                    }
+                    umma_commit(&kv_empty[vat % kStages]);
+                    if (j + 1 < it.most)
+                        umma_commit(&kv_empty[kat % kStages]);
+                    if (j + 2 == it.most)
+                        umma_commit(q_empty);
+                }
+            }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, fine);
+            p_phase[0] += it.n[0];
+            p_phase[1] += it.n[1];
+            place += 2 * it.most;
+            ++blocks;
+        }
+        if (elect_one()) { // every product, and every arrival that one of them still owes, before the block ends
+            umma_commit(drain);
+            mbar_wait_bounded(drain, 0, a.status, STATUS_TIMEOUT_MMA);
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- V tiles that are not seen to the end
+        const int half = warp - 10;
+        int place = 0, blocks = 0;
+        uint32_t edges = 0;
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            const PaItem it = pa_item(a, number(round), lane);
+            if (!it.valid)
+                break;
+            if (it.most == 0)
+                continue;
+            int bad = 0;
+            for (int j = it.edge; j < it.most; ++j) {
+                const int s = (place + pa_v_place(j, it.most)) % kStages;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&edge_full[s], edges >> s & 1, a.status, STATUS_TIMEOUT_TMA));
+                if (!ok)
+                    break;
+                edges ^= 1u << s;
+                uint8_t *tile = ring + s * kTile + half * 64 * 128;
+#pragma unroll 1
+                for (int h = 0; h < kHalves; ++h) {
+#pragma unroll 4
+                    for (int i = 0; i < 64 * 128 / (32 * 16); ++i) {
+                        uint4 *p = reinterpret_cast<uint4 *>(tile + h * kHalf + (i * 32 + lane) * 16);
+                        uint4 x = *p;
+                        uint32_t w[4] = { x.x, x.y, x.z, x.w }, top = 0;
+                        constexpr uint32_t kOne = BF16 ? 0x00800080u : 0x04000400u; // the exponent's lowest bit: a full exponent carries into bit 15
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            top |= ((w[e] & 0x7fff7fffu) + kOne) & 0x80008000u;
+                        if (top) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t f = ((w[e] & 0x7fff7fffu) + kOne) & 0x80008000u;
+                                w[e] &= ~((f >> 15) * 0xffffu);
+                            }
+                            *p = make_uint4(w[0], w[1], w[2], w[3]);
+                            const int key = j * kPaKeys + half * 64 + ((i * 32 + lane) >> 3);
+                            bad |= key < it.nk;
+                        }
+                    }
+                }
+                bad = __any_sync(0xffffffffu, bad);
+                if (j == it.most - 1 && lane == 0)
+                    poison[4 * half + (blocks & 3)] = bad; // (copies run at most two blocks ahead of the softmax)
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&kv_full[s]);
+            }
+            place += 2 * it.most;
+            ++blocks;
+        }
+    }
+
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+static int pack_log2_of(int group) // the largest power of two that divides the group, at most 16
+{
+    int p = 0;
+    while (p < 4 && group % (2 << p) == 0)
+        ++p;
+    return p;
+}
+
+static bool map_rows(CUtensorMap *m, const void *base, int D, int heads, int rows, long long head_stride, long long stride, int box_heads, int box_rows)
+{
+    const uint64_t dims[3] = { (uint64_t)D * 2, (uint64_t)heads, (uint64_t)rows };
+    // (a dimension of one may come with any stride)
+    const uint64_t strides[2] = { (uint64_t)(heads > 1 ? 2 * head_stride : 2 * D), (uint64_t)(rows > 1 ? 2 * stride : 2 * D) };
+    const uint32_t box[3] = { 128, (uint32_t)box_heads, (uint32_t)box_rows };
+    return encode_tmap(m, TMAP_U8, 3, base, dims, strides, box, TMAP_SWIZZLE_128B);
+}
+
+template <int D, bool BF16>
+static cudaError_t launch_prompt(const CUtensorMap *m, const PaArgs &a, unsigned grid, cudaStream_t stream)
+{
+    static thread_local SmemOptIn opted;
+    auto kern = prompt_attention_kernel<D, BF16>;
+    const cudaError_t e = opted.ensure(kern, PaShape<D>::kSmem);
+    if (e != cudaSuccess)
+        return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kPaThreads);
+    cfg.dynamicSmemBytes = PaShape<D>::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, m[0], m[1], m[2], a);
+}
+
+static bool strides_positive(int rows, int heads, long long stride, long long head_stride)
+{
+    return (rows <= 1 || (stride > 0 && stride < (1ll << 38))) && (heads <= 1 || (head_stride > 0 && head_stride < (1ll << 38)));
+}
+
+} // namespace abq
+
+extern "C" abq_status abq_prompt_attention(const abq_prompt_attention_params *p, abq_stream_t stream)
+{
+    using namespace abq;
+    if (!p || p->total_q < 0 || p->total_k < 0 || p->batch < 0 || p->kv_heads <= 0 || p->q_heads <= 0 || p->q_heads % p->kv_heads || p->q_heads > 65536 ||
+        (p->head_dim != 64 && p->head_dim != 128) || (p->half_type != ABQ_HALF_FP16 && p->half_type != ABQ_HALF_BF16) || p->max_q < 0 ||
+        !(p->scale > 0.f && p->scale <= 2e38f) || (reinterpret_cast<uintptr_t>(p->status_word) & 3))
+        return ABQ_ERR_INVALID_ARG;
+    if (p->total_q == 0 || p->batch == 0)
+        return ABQ_OK;
+    if (!half_rows_valid(p->q, p->q_stride, p->q_head_stride) || !half_rows_valid(p->out, p->out_stride, p->out_head_stride) ||
+        !strides_positive(p->total_q, p->q_heads, p->q_stride, p->q_head_stride) || !strides_positive(p->total_q, p->q_heads, p->out_stride, p->out_head_stride) ||
+        !p->cu_q || !p->cu_k || ((reinterpret_cast<uintptr_t>(p->cu_q) | reinterpret_cast<uintptr_t>(p->cu_k)) & 3))
+        return ABQ_ERR_INVALID_ARG;
+    if (p->total_k > 0 && (!half_rows_valid(p->k, p->k_stride, p->k_head_stride) || !half_rows_valid(p->v, p->v_stride, p->v_head_stride) ||
+                           !strides_positive(p->total_k, p->kv_heads, p->k_stride, p->k_head_stride) || !strides_positive(p->total_k, p->kv_heads, p->v_stride, p->v_head_stride)))
+        return ABQ_ERR_INVALID_ARG;
+    if (p->out == p->q && (p->out_stride != p->q_stride || p->out_head_stride != p->q_head_stride))
+        return ABQ_ERR_INVALID_ARG;
+    const int group = p->q_heads / p->kv_heads, pl = pack_log2_of(group), D = p->head_dim;
+    const long long head_groups = p->q_heads >> pl, tokens = 256 >> pl;
+    long long slots = p->total_q / tokens + p->batch; // each sequence at most one block that is not full
+    if (p->max_q)
+        slots = std::min<long long>(slots, p->batch * ((p->max_q + tokens - 1) / tokens));
+    if (slots * head_groups + 2048 >= (1ll << 31))
+        return ABQ_ERR_INVALID_ARG;
+    CUtensorMap m[3];
+    const void *k = p->total_k ? p->k : p->q, *v = p->total_k ? p->v : p->q; // (without a key nothing is read)
+    const int rows_k = p->total_k ? p->total_k : 1, heads_k = p->total_k ? p->kv_heads : 1;
+    if (!map_rows(&m[0], p->q, D, p->q_heads, p->total_q, p->q_head_stride, p->q_stride, 1 << pl, 128 >> pl) ||
+        !map_rows(&m[1], k, D, heads_k, rows_k, p->k_head_stride, p->k_stride, 1, kPaKeys) || !map_rows(&m[2], v, D, heads_k, rows_k, p->v_head_stride, p->v_stride, 1, kPaKeys))
+        return ABQ_ERR_CUDA;
+    PaArgs a = {};
+    a.cu_q = p->cu_q, a.cu_k = p->cu_k, a.v = reinterpret_cast<const uint8_t *>(p->v), a.out = reinterpret_cast<uint8_t *>(p->out);
+    a.v_stride = 2 * p->v_stride, a.v_head_stride = 2 * p->v_head_stride, a.out_stride = 2 * p->out_stride, a.out_head_stride = 2 * p->out_head_stride;
+    a.total_q = p->total_q, a.total_k = p->total_k, a.batch = p->batch, a.head_groups = (int)head_groups, a.pack_log2 = pl, a.group = group;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.status = p->status_word;
+    const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(148, slots * head_groups));
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const bool bf16 = p->half_type == ABQ_HALF_BF16;
+    const cudaError_t e = D == 128 ? (bf16 ? launch_prompt<128, true>(m, a, grid, s) : launch_prompt<128, false>(m, a, grid, s))
+                                   : (bf16 ? launch_prompt<64, true>(m, a, grid, s) : launch_prompt<64, false>(m, a, grid, s));
+    if (e != cudaSuccess) {
+        set_last_cuda_error(e);
+        return ABQ_ERR_CUDA;
+    }
+    return ABQ_OK;
+}

@@ -439,6 +439,29 @@ typedef struct abq_cache_attention_params {
 ABQ_API size_t abq_cache_attention_workspace_bytes(const abq_kv_cache *cache, int batch, int rows_per_seq, int q_heads);
 ABQ_API abq_status abq_cache_attention(const abq_cache_attention_params *params, abq_stream_t stream);
 
+/*
+ * Causal attention of whole prompts, packed behind one another: rows cu_q[b] .. cu_q[b + 1] - 1 of q and out belong to sequence b, rows cu_k[b] .. of k and v
+ * are its keys and values.  Row i of a sequence of n queries and m keys sees keys 0 .. i + m - n: with m > n the queries are the last of the
+ * keys' tokens (a chunk of a prompt behind its prefix), and a row that sees no key (m < n) gives 0.  Rows of `out` from cu_q[batch] on are left as
+ * they were.  Keys and values that a row does not see may hold anything, Inf and NaN included.  Products run on the tensor cores in the 16-bit type, sums and
+ * the softmax in fp32; p is rounded to the 16-bit type.
+ * Strides of dimensions longer than one are positive.  The call reads nothing back and allocates nothing; it may be captured.
+ */
+typedef struct abq_prompt_attention_params {
+    const void *q, *k, *v; /* [total_q][q_heads][head_dim], [total_k][kv_heads][head_dim] */
+    void *out;             /* [total_q][q_heads][head_dim]; may be q itself */
+    long long q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, out_stride, out_head_stride;
+    int total_q, total_k;  /* rows that the arrays hold; ends beyond them are cut */
+    int q_heads, kv_heads, head_dim;
+    int half_type;         /* abq_half_type of all four */
+    int batch;
+    const int *cu_q, *cu_k; /* device int32 [batch + 1], starting at 0, never falling */
+    int max_q;             /* rows of the longest sequence where known, or 0: sizes the launch, changes no result */
+    float scale;           /* positive */
+    int *status_word;      /* optional */
+} abq_prompt_attention_params;
+ABQ_API abq_status abq_prompt_attention(const abq_prompt_attention_params *params, abq_stream_t stream);
+
 /* Text for a status code; cudaError_t of the last failing CUDA call in this thread (0 if none). */
 ABQ_API const char *abq_status_string(abq_status s);
 ABQ_API int abq_last_cuda_error(void);

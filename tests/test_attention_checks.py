@@ -12,7 +12,7 @@ INVALID, WORKSPACE = 1, 3
 
 def test_struct_sizes_match_the_header(abq, tmp_path):
     names = {"abq_kv_cache": abq.KVCache, "abq_kv_write_params": abq.KVWriteParams, "abq_kv_read_params": abq.KVReadParams,
-             "abq_cache_attention_params": abq.CacheAttentionParams}
+             "abq_cache_attention_params": abq.CacheAttentionParams, "abq_prompt_attention_params": abq.PromptAttentionParams}
     src = tmp_path / "sz.c"
     src.write_text('#include "abq_b200.h"\n#include <stdio.h>\nint main(void){' + "".join(f'printf("%zu\\n", sizeof({n}));' for n in names) + "return 0;}\n")
     subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "sz")], check=True)
@@ -81,6 +81,22 @@ def test_cache_attention_refuses(abq):
     for rows, heads in ((0, 4), (65, 4), (1, 3), (1, 0)):
         assert abq.cache_attention_workspace_bytes(c, 2, rows, heads) == 0
     assert abq.cache_attention_workspace_bytes(c, 2, 16, 4) > abq.cache_attention_workspace_bytes(c, 2, 8, 4) > need
+
+
+def test_prompt_attention_refuses(abq):
+    good = dict(q=4096, k=4096, v=4096, out=8192, q_stride=512, q_head_stride=128, k_stride=256, k_head_stride=128, v_stride=256, v_head_stride=128, out_stride=512,
+                out_head_stride=128, total_q=10, total_k=10, q_heads=4, kv_heads=2, head_dim=128, half_type=0, batch=2, cu_q=4096, cu_k=4096, scale=0.1)
+    fn = abq.lib().abq_prompt_attention
+    _refused(fn, abq.PromptAttentionParams, good,
+             [dict(q=None), dict(q=4104), dict(k=None), dict(v=4098), dict(out=None), dict(out=8200), dict(q_stride=4), dict(k_head_stride=129), dict(v_stride=-256), dict(out_stride=0),
+              dict(k_stride=0), dict(q_heads=3), dict(q_heads=0), dict(kv_heads=0), dict(head_dim=96), dict(half_type=2), dict(batch=-1), dict(total_q=-1), dict(total_k=-1),
+              dict(cu_q=None), dict(cu_k=4098), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(max_q=-1), dict(status_word=4097),
+              dict(out=4096, out_stride=1024)])
+    for empty in (dict(total_q=0), dict(batch=0)):
+        p = abq.PromptAttentionParams()
+        for k, v in {**good, **empty}.items():
+            setattr(p, k, v)
+        assert fn(ctypes.byref(p), None) == 0  # nothing to do
 
 
 def test_python_layer_refuses(abq):
