@@ -1,16 +1,20 @@
 // C entry of the attention over the quantised cache: checks, row blocks and grid (the kernels are in cache_attention.cuh).
+#include <algorithm>
+
 #include "cache_attention.cuh"
 
 namespace abq {
 
 template <int NT>
-cudaError_t launch_cache_attention(const CacheAttnArgs &args, int head_dim, int bits, cudaStream_t stream);
-extern template cudaError_t launch_cache_attention<1>(const CacheAttnArgs &, int, int, cudaStream_t);
-extern template cudaError_t launch_cache_attention<2>(const CacheAttnArgs &, int, int, cudaStream_t);
-extern template cudaError_t launch_cache_attention<4>(const CacheAttnArgs &, int, int, cudaStream_t);
+cudaError_t launch_cache_attention(const CacheAttnArgs &args, int head_dim, int bits, bool bf16, cudaStream_t stream);
+extern template cudaError_t launch_cache_attention<1>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
+extern template cudaError_t launch_cache_attention<2>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
+extern template cudaError_t launch_cache_attention<4>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
 
 // Tiles of 8 query rows that a block holds: one conversion of the codes serves them all; 32 rows are what the registers hold.
 static int row_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
+static int most_runs(int tiles) { return kCaSms * ca_ctas_per_sm(tiles) * kCaWarps; }
 
 static bool attention_shape_valid(const abq_kv_cache &c, int batch, int n, int q_heads)
 {
@@ -26,8 +30,8 @@ extern "C" size_t abq_cache_attention_workspace_bytes(const abq_kv_cache *cache,
     using namespace abq;
     if (!cache || !attention_shape_valid(*cache, batch, rows_per_seq, q_heads))
         return 0;
-    const int rows = 8 * row_tiles(rows_per_seq * (q_heads / cache->kv_heads));
-    return (size_t)2 * kCaMaxCtas * rows * (cache->head_dim + 2) * sizeof(float);
+    const int rows = rows_per_seq * (q_heads / cache->kv_heads), tiles = row_tiles(rows);
+    return (size_t)2 * most_runs(tiles) * std::min(rows, 8 * tiles) * (cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, abq_stream_t stream)
@@ -53,16 +57,20 @@ extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, a
     a.q_stride = 2 * p->q_stride, a.q_head_stride = 2 * p->q_head_stride, a.out_stride = 2 * p->out_stride, a.out_head_stride = 2 * p->out_head_stride;
     a.table = p->block_table, a.seq_lens = p->seq_lens, a.tree = p->tree, a.part = reinterpret_cast<float *>(p->workspace), a.status = p->status_word;
     a.num_pages = p->cache.num_pages, a.page_granules = p->cache.page_size / 16, a.kv_heads = p->cache.kv_heads, a.batch = p->batch, a.n = p->rows_per_seq;
-    a.group = p->q_heads / p->cache.kv_heads, a.table_stride = p->table_stride, a.bf16 = p->cache.half_type == ABQ_HALF_BF16;
+    a.group = p->q_heads / p->cache.kv_heads, a.table_stride = p->table_stride;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     const int rows = a.n * a.group, tiles = row_tiles(rows);
     a.row_blocks = (rows + 8 * tiles - 1) / (8 * tiles);
+    a.slot_rows = std::min(rows, 8 * tiles);
     // the longest sequences that the tables can hold bound the work; real lengths are read on the device
-    const long long most = (long long)a.batch * a.kv_heads * a.row_blocks * a.table_stride * a.page_granules;
-    a.ctas = (int)(most < (long long)kCaMaxCtas * kCaMinQuota ? (most + kCaMinQuota - 1) / kCaMinQuota : kCaMaxCtas);
+    const long long most = (long long)a.batch * a.kv_heads * a.row_blocks * ((long long)a.table_stride * a.page_granules + kCaExtra);
+    a.runs = (int)std::min<long long>((most + kCaMinQuota - 1) / kCaMinQuota, most_runs(tiles));
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int D = p->cache.head_dim, bits = p->cache.bits;
-    const cudaError_t e = tiles == 1 ? launch_cache_attention<1>(a, D, bits, s) : tiles == 2 ? launch_cache_attention<2>(a, D, bits, s) : launch_cache_attention<4>(a, D, bits, s);
+    const bool bf16 = p->cache.half_type == ABQ_HALF_BF16;
+    const cudaError_t e = tiles == 1   ? launch_cache_attention<1>(a, D, bits, bf16, s)
+                          : tiles == 2 ? launch_cache_attention<2>(a, D, bits, bf16, s)
+                                       : launch_cache_attention<4>(a, D, bits, bf16, s);
     if (e != cudaSuccess) {
         set_last_cuda_error(e);
         return ABQ_ERR_CUDA;

@@ -4,12 +4,12 @@
 
 namespace abq {
 
-template <typename Kernel>
-cudaError_t launch_chained(Kernel kern, unsigned grid, unsigned block, size_t smem, cudaStream_t stream, const CacheAttnArgs &args)
+template <typename Kernel, typename... Args>
+cudaError_t launch_chained(Kernel kern, dim3 grid, size_t smem, cudaStream_t stream, const Args &...args)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kCaThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -17,29 +17,39 @@ cudaError_t launch_chained(Kernel kern, unsigned grid, unsigned block, size_t sm
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, args);
+    return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <int D, int BITS, int NT>
+template <int D, int BITS, int NT, bool BF16>
 cudaError_t launch_cache_attention_as(const CacheAttnArgs &args, cudaStream_t stream)
 {
     static thread_local SmemOptIn opted;
     constexpr int smem = CaShape<D, BITS, NT>::kSmem;
-    auto kern = cache_attention_kernel<D, BITS, NT>;
+    auto kern = cache_attention_kernel<D, BITS, NT, BF16>;
     cudaError_t e = opted.ensure(kern, smem);
     if (e == cudaSuccess)
-        e = launch_chained(kern, args.ctas, kCaThreads, smem, stream, args);
-    if (e == cudaSuccess)
-        e = launch_chained(cache_attention_combine_kernel<D, NT>, (unsigned)(args.batch * args.kv_heads * args.row_blocks), kCaThreads, 0, stream, args);
-    return e;
+        e = launch_chained(kern, dim3((args.runs + kCaWarps - 1) / kCaWarps), smem, stream, args);
+    if (e != cudaSuccess)
+        return e;
+    constexpr int kGroups = kCaThreads / (D / 8);
+    int rows = 1; // of a block at a time
+    while (rows < args.slot_rows && rows < kGroups)
+        rows *= 2;
+    return launch_chained(cache_attention_combine_kernel<D, BF16>, dim3(args.batch * args.kv_heads * args.row_blocks, (args.slot_rows + rows - 1) / rows), 0, stream, args, 8 * NT,
+                          rows);
 }
 
 template <int NT>
-cudaError_t launch_cache_attention(const CacheAttnArgs &args, int head_dim, int bits, cudaStream_t stream)
+cudaError_t launch_cache_attention(const CacheAttnArgs &args, int head_dim, int bits, bool bf16, cudaStream_t stream)
 {
-    if (head_dim == 128)
-        return bits == 8 ? launch_cache_attention_as<128, 8, NT>(args, stream) : launch_cache_attention_as<128, 4, NT>(args, stream);
-    return bits == 8 ? launch_cache_attention_as<64, 8, NT>(args, stream) : launch_cache_attention_as<64, 4, NT>(args, stream);
+    if (head_dim == 128) {
+        if (bits == 8)
+            return bf16 ? launch_cache_attention_as<128, 8, NT, true>(args, stream) : launch_cache_attention_as<128, 8, NT, false>(args, stream);
+        return bf16 ? launch_cache_attention_as<128, 4, NT, true>(args, stream) : launch_cache_attention_as<128, 4, NT, false>(args, stream);
+    }
+    if (bits == 8)
+        return bf16 ? launch_cache_attention_as<64, 8, NT, true>(args, stream) : launch_cache_attention_as<64, 8, NT, false>(args, stream);
+    return bf16 ? launch_cache_attention_as<64, 4, NT, true>(args, stream) : launch_cache_attention_as<64, 4, NT, false>(args, stream);
 }
 
 } // namespace abq

@@ -2,5 +2,5 @@
 #include "cache_attention_launch.cuh"
 
 namespace abq {
-template cudaError_t launch_cache_attention<2>(const CacheAttnArgs &, int head_dim, int bits, cudaStream_t stream);
+template cudaError_t launch_cache_attention<2>(const CacheAttnArgs &, int head_dim, int bits, bool bf16, cudaStream_t stream);
 }

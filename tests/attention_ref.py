@@ -89,7 +89,8 @@ def cache_attention(data, page_size, bits, half, table, lens, q, n, scale, tree=
     """(result, error bound) in float64 for 16-bit q [batch * n][q_heads][dim]; everything on the CPU.
 
     The bound: the result's own rounding (half a step); p vs rounded to fp16 (2^-11 of p vs |c'|, and what underflows below 2^-39 of the
-    largest); the score's error d, at most 2^-20 of scale log2(e) sum|q| (2^(bits-1) ks + |ko|) (8 products of 16 and the joining terms in fp32, 2^-23 each),
+    largest); the score's error d: the codes c are multiplied as o + c (o = 1024 for 8 bits, 64 for 4) in 8 products of 16 and joined with sum(q) (km - o ks), in fp32,
+    2^-23 each, so at most 2^-20 of scale log2(e) sum|q| ((o + 2^bits) ks + |km - o ks|),
     plus, for bf16 queries, what the scaled fp16 row loses below its 2^-14 (2^-25 of twice the row's largest per feature), which moves p and the sum of p by
     at most 2 ln 2 d each; sums of p and of p v in fp32 with the exponential's 2^-22, 2^-18 of the sum of magnitudes together."""
     dim, heads = q.shape[2], q.shape[1]
@@ -116,7 +117,8 @@ def cache_attention(data, page_size, bits, half, table, lens, q, n, scale, tree=
         out[b * n:(b + 1) * n] = got.permute(2, 0, 1, 3).reshape(n, heads, dim)
         mags = torch.where(seen.any(0).view(1, -1, 1), vs * centre + (vm + centre * vs).abs(), torch.zeros_like(vs)).nan_to_num(0.0)
         codes = torch.where(seen.any(0).view(1, -1, 1), vs * (vc - centre).abs(), torch.zeros_like(vc)).nan_to_num(0.0)
-        kmag = (ks * centre + (km + centre * ks).abs()).nan_to_num(0.0).amax((1, 2)).view(H, 1, 1, 1)
+        o = 1024.0 if bits == 8 else 64.0
+        kmag = (ks * (o + 2.0 ** bits) + (km - o * ks).abs()).nan_to_num(0.0).amax((1, 2)).view(H, 1, 1, 1)
         qsum = qq.abs().sum(-1, keepdim=True) * 2.0 ** -20
         if half == torch.bfloat16:
             qsum = qsum + qq.abs().amax(-1, keepdim=True) * dim * 2.0 ** -24
