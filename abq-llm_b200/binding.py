@@ -184,6 +184,25 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream
 
 
+def _raw_stream(stream):
+    """As _stream(), without making a Stream object for the current one where torch has a way to (a call of a few microseconds shows the difference)."""
+    if stream is not None:
+        return _stream(stream)
+    global _current_raw
+    if _current_raw is None:
+        import torch
+        get, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+        if get is None or device is None:
+            _current_raw = lambda: _stream(None)  # noqa: E731
+        else:
+            torch.cuda.current_stream()  # (initialises CUDA)
+            _current_raw = lambda: get(device())  # noqa: E731
+    return _current_raw()
+
+
+_current_raw = None
+
+
 def _check(status: int, what: str) -> None:
     if status != 0:
         extra = ""
@@ -387,7 +406,9 @@ def make_kv_write_params(cache: KVCache, k, v, slots) -> KVWriteParams:
 
 
 def kv_cache_write(params: KVWriteParams, stream=None) -> None:
-    _check(lib().abq_kv_cache_write(ctypes.byref(params), _stream(stream)), "abq_kv_cache_write")
+    status = (_lib or lib()).abq_kv_cache_write(ctypes.byref(params), _raw_stream(stream))
+    if status:
+        _check(status, "abq_kv_cache_write")
 
 
 def make_kv_read_params(cache: KVCache, k, v, block_table, cu_seqlens) -> KVReadParams:
@@ -406,7 +427,9 @@ def make_kv_read_params(cache: KVCache, k, v, block_table, cu_seqlens) -> KVRead
 
 
 def kv_cache_read(params: KVReadParams, stream=None) -> None:
-    _check(lib().abq_kv_cache_read(ctypes.byref(params), _stream(stream)), "abq_kv_cache_read")
+    status = (_lib or lib()).abq_kv_cache_read(ctypes.byref(params), _raw_stream(stream))
+    if status:
+        _check(status, "abq_kv_cache_read")
 
 
 def cache_attention_workspace_bytes(cache: KVCache, batch: int, rows_per_seq: int, q_heads: int) -> int:
@@ -435,7 +458,9 @@ def make_cache_attention_params(cache: KVCache, q, out, block_table, seq_lens, *
 
 
 def cache_attention(params: CacheAttentionParams, stream=None) -> None:
-    _check(lib().abq_cache_attention(ctypes.byref(params), _stream(stream)), "abq_cache_attention")
+    status = (_lib or lib()).abq_cache_attention(ctypes.byref(params), _raw_stream(stream))
+    if status:
+        _check(status, "abq_cache_attention")
 
 
 def make_prompt_attention_params(q, k, v, out, cu_q, cu_k, *, scale: float, max_q: int = 0, status_word=None) -> PromptAttentionParams:
@@ -458,4 +483,6 @@ def make_prompt_attention_params(q, k, v, out, cu_q, cu_k, *, scale: float, max_
 
 
 def prompt_attention(params: PromptAttentionParams, stream=None) -> None:
-    _check(lib().abq_prompt_attention(ctypes.byref(params), _stream(stream)), "abq_prompt_attention")
+    status = (_lib or lib()).abq_prompt_attention(ctypes.byref(params), _raw_stream(stream))
+    if status:
+        _check(status, "abq_prompt_attention")

@@ -635,16 +635,29 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1)
             top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
-#pragma unroll 4
-        for (int c = c0 + turn; c <= c1; c += turns) {
-            const size_t slot = slot_of(c) * a.slot_rows + row;
-            const float2 p = ml[slot];
-            const float f = p.x == -INFINITY ? 1.f : ex2(p.x - top);
-            lsum = fmaf(f, p.y, lsum);
-            const float *src = a.part + slot * D + sub * 8;
-            const float4 lo = *reinterpret_cast<const float4 *>(src), hi = *reinterpret_cast<const float4 *>(src + 4);
-            v[0] = fmaf(f, lo.x, v[0]), v[1] = fmaf(f, lo.y, v[1]), v[2] = fmaf(f, lo.z, v[2]), v[3] = fmaf(f, lo.w, v[3]);
-            v[4] = fmaf(f, hi.x, v[4]), v[5] = fmaf(f, hi.y, v[5]), v[6] = fmaf(f, hi.z, v[6]), v[7] = fmaf(f, hi.w, v[7]);
+        for (int c = c0 + turn; c <= c1; c += 4 * turns) { // four pieces under way
+            float2 p[4];
+            float4 lo[4], hi[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int at = c + u * turns;
+                p[u] = make_float2(-INFINITY, 0.f);
+                lo[u] = hi[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at <= c1) {
+                    const size_t slot = slot_of(at) * a.slot_rows + row;
+                    const float *src = a.part + slot * D + sub * 8;
+                    p[u] = ml[slot];
+                    lo[u] = *reinterpret_cast<const float4 *>(src);
+                    hi[u] = *reinterpret_cast<const float4 *>(src + 4);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float f = p[u].x == -INFINITY ? 1.f : ex2(p[u].x - top);
+                lsum = fmaf(f, p[u].y, lsum);
+                v[0] = fmaf(f, lo[u].x, v[0]), v[1] = fmaf(f, lo[u].y, v[1]), v[2] = fmaf(f, lo[u].z, v[2]), v[3] = fmaf(f, lo[u].w, v[3]);
+                v[4] = fmaf(f, hi[u].x, v[4]), v[5] = fmaf(f, hi[u].y, v[5]), v[6] = fmaf(f, hi[u].z, v[6]), v[7] = fmaf(f, hi[u].w, v[7]);
+            }
         }
     }
     if (turns > 1) {

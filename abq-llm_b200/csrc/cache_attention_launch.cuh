@@ -32,11 +32,12 @@ cudaError_t launch_cache_attention_as(const CacheAttnArgs &args, cudaStream_t st
     if (e != cudaSuccess)
         return e;
     constexpr int kGroups = kCaThreads / (D / 8);
-    int rows = 1; // of a block at a time
-    while (rows < args.slot_rows && rows < kGroups)
+    // rows of a block at a time: few (the other groups of threads take pieces in turn) where the items alone do not fill the GPU
+    const long long items = (long long)args.batch * args.kv_heads * args.row_blocks;
+    int rows = 1;
+    while (rows < args.slot_rows && rows < kGroups && items * args.slot_rows / rows > 4 * kCaSms)
         rows *= 2;
-    return launch_chained(cache_attention_combine_kernel<D, BF16>, dim3(args.batch * args.kv_heads * args.row_blocks, (args.slot_rows + rows - 1) / rows), 0, stream, args, 8 * NT,
-                          rows);
+    return launch_chained(cache_attention_combine_kernel<D, BF16>, dim3((unsigned)items, (args.slot_rows + rows - 1) / rows), 0, stream, args, 8 * NT, rows);
 }
 
 template <int NT>

@@ -5,9 +5,12 @@
 // shuffles on a packed (min, -max) pair.  A CTA takes 16 consecutive tokens, so that the rows of a granule and its 64-byte parameter lines are
 // touched by one CTA, and several heads one after the other, keys and values of one head in flight together.
 //
-// Quantiser: code = rint((x - min) / scale), a correctly rounded fp32 division.  It is taken as a product with the reciprocal: that is off by at most
-// 2^-23 of a quotient of at most 255.5, 3.1e-5, so a quotient further than 2^-14 from the middle between two codes rounds to the same one;
-// the others (and rows whose scale is below the normal range) are divided.  The scale is rounded up to 16 bits, so max never passes the last code.
+// Quantiser: code = rint((x - min) / scale), a correctly rounded fp32 division.  It is taken twice as a product with the reciprocal, made 2^-20 too small and
+// too large, in one multiply-add that rounds to an integer: where both give the same code the division does too; a row part where they do not (a quotient
+// close to the middle between two codes), or whose scale is below the normal range, is divided.  The scale is rounded up to 16 bits, so max never passes the
+// last code.
+#include <type_traits>
+
 #include "abq_kernels.h"
 #include "kv_cache.cuh"
 
@@ -19,7 +22,6 @@ struct KvShape {
     uint8_t *data;
     long long capacity; // places: num_pages * page_size
     int num_pages, page_size, kv_heads;
-    bool bf16;
 };
 
 __device__ __forceinline__ uint8_t *kv_granule(const KvShape &c, int page, int place, int head, int granule_bytes)
@@ -27,66 +29,89 @@ __device__ __forceinline__ uint8_t *kv_granule(const KvShape &c, int page, int p
     return c.data + (((size_t)page * c.kv_heads + head) * (c.page_size >> 4) + (place >> 4)) * granule_bytes;
 }
 
-// The lesser (min, -max) of two packed pairs, NaN ignored
-__device__ __forceinline__ uint32_t range_min(uint32_t a, uint32_t b, bool bf16)
+// The lesser and the larger of two packed pairs; NaN stays
+template <bool BF16>
+__device__ __forceinline__ uint32_t pair_min(uint32_t a, uint32_t b)
 {
-    if (bf16) {
-        const __nv_bfloat162 r = __hmin2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    const __half2 r = __hmin2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
-    return *reinterpret_cast<const uint32_t *>(&r);
+    uint32_t r;
+    if (BF16)
+        asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    if (BF16)
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pack_floats(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack_bits(uint64_t v, uint32_t &lo, uint32_t &hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t add_floats(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_floats(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
-template <int D, int BITS>
-__device__ __forceinline__ void quantise_row(const uint4 &x, int sub, int place, uint8_t *granule, int part, bool bf16, bool kept)
+template <int D, int BITS, bool BF16>
+__device__ __forceinline__ void quantise_row(const uint4 &x, int sub, int place, uint8_t *granule, int part, bool kept)
 {
     constexpr int RB = kv_row_bytes(D, BITS), kLanes = D / 8;
     const uint32_t w[4] = { x.x, x.y, x.z, x.w };
-    uint32_t lo = w[0], neg = w[0] ^ 0x80008000u, mag = w[0] & 0x7fff7fffu; // lo: mins of even and odd values, neg: mins of their negatives
+    const uint32_t lo = pair_min<BF16>(pair_min<BF16>(w[0], w[1]), pair_min<BF16>(w[2], w[3]));
+    const uint32_t hi = pair_max<BF16>(pair_max<BF16>(w[0], w[1]), pair_max<BF16>(w[2], w[3])) ^ 0x80008000u;
+    uint32_t range = pair_min<BF16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632)); // (min, -max)
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-        lo = range_min(lo, w[i], bf16);
-        neg = range_min(neg, w[i] ^ 0x80008000u, bf16);
-        mag = __vmaxu2(mag, w[i] & 0x7fff7fffu);
-    }
-    // (min of all, min of negatives) in one word, and the largest magnitude's bits for the check on Inf and NaN
-    uint32_t range = range_min(__byte_perm(lo, neg, 0x5410), __byte_perm(lo, neg, 0x7632), bf16);
-    uint32_t top = max(mag & 0xffffu, mag >> 16);
-#pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) {
-        range = range_min(range, __shfl_xor_sync(0xffffffffu, range, o), bf16);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    const float2 mm = half_pair_to_float(range, bf16);
+    for (int o = 1; o < kLanes; o <<= 1)
+        range = pair_min<BF16>(range, __shfl_xor_sync(0xffffffffu, range, o));
+    const float2 mm = half_pair_to_float(range, BF16);
     const float mn = mm.x, spread = -mm.y - mm.x;
-    const bool finite = top < (bf16 ? 0x7f80u : 0x7c00u) && spread <= 3.402823466e38f;
+    const bool finite = spread <= 3.402823466e38f; // (not for Inf or NaN among the values)
     const float fine = spread / (float)((1 << BITS) - 1);
-    uint32_t sbits = float_pair_to_half(fine, 0.f, bf16) & 0xffffu;
-    if (half_bits_to_float(sbits, bf16) < fine)
+    uint32_t sbits = float_pair_to_half(fine, 0.f, BF16) & 0xffffu;
+    if (half_bits_to_float(sbits, BF16) < fine)
         ++sbits; // up to the next 16-bit value (positive values are ordered like their bits)
-    const float s = half_bits_to_float(sbits, bf16);
-    const bool usual = s >= 1.17549435e-38f; // the reciprocal of a normal number is finite
-    const float inv = usual ? 1.f / s : 0.f;
-    uint32_t code[8];
-    bool close = s > 0.f && !usual;
-    const float magic = 12582912.f; // 1.5 * 2^23: the sum's low bits are the rounded value
+    const float s = half_bits_to_float(sbits, BF16);
+    float inv;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s)); // at most 1 ulp off
+    const bool usual = s >= 1.17549435e-38f && s <= 8.5e37f; // the reciprocal is a normal number
+    inv = usual ? inv : 0.f;
+    const float less = inv * (1.f - 9.5367432e-7f), more = inv * (1.f + 9.5367432e-7f);
+    const uint64_t less2 = pack_floats(less, less), more2 = pack_floats(more, more), mn2 = pack_floats(-mn, -mn);
+    const uint64_t magic2 = pack_floats(12582912.f, 12582912.f); // 1.5 * 2^23: the sum's low bits are the rounded value
+    uint32_t code[8], differ = s > 0.f && !usual;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 f = half_pair_to_float(w[i], bf16);
-        const float t0 = (f.x - mn) * inv, t1 = (f.y - mn) * inv;
-        const float r0 = t0 + magic, r1 = t1 + magic;
-        close |= fabsf(t0 - (r0 - magic)) > 0.5f - 6.1035156e-5f;
-        close |= fabsf(t1 - (r1 - magic)) > 0.5f - 6.1035156e-5f;
-        code[2 * i] = __float_as_uint(r0);
-        code[2 * i + 1] = __float_as_uint(r1);
+        const float2 f = half_pair_to_float(w[i], BF16);
+        const uint64_t d = add_floats(pack_floats(f.x, f.y), mn2);
+        uint32_t m0, m1;
+        unpack_bits(fma_floats(d, less2, magic2), code[2 * i], code[2 * i + 1]);
+        unpack_bits(fma_floats(d, more2, magic2), m0, m1);
+        differ |= (code[2 * i] ^ m0) | (code[2 * i + 1] ^ m1);
     }
-    if (close) {
+    if (differ) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = half_pair_to_float(w[i], bf16);
-            code[2 * i] = (uint32_t)__float2int_rn((f.x - mn) / s);
-            code[2 * i + 1] = (uint32_t)__float2int_rn((f.y - mn) / s);
+            const float2 f = half_pair_to_float(w[i], BF16);
+            code[2 * i] = s > 0.f ? (uint32_t)__float2int_rn((f.x - mn) / s) : 0u;
+            code[2 * i + 1] = s > 0.f ? (uint32_t)__float2int_rn((f.y - mn) / s) : 0u;
         }
     }
     if (!finite) {
@@ -104,14 +129,15 @@ __device__ __forceinline__ void quantise_row(const uint4 &x, int sub, int place,
         o.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
         *reinterpret_cast<uint2 *>(rows + kv_place<RB>(t, sub * 8)) = o;
     } else {
-        uint32_t o = 0;
+        uint32_t two[4]; // the low byte: two codes
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            o |= (code[i] & 15u) << (4 * i);
+        for (int i = 0; i < 4; ++i)
+            two[i] = code[2 * i] + (code[2 * i + 1] << 4);
+        const uint32_t o = __byte_perm(__byte_perm(two[0], two[1], 0x0040), __byte_perm(two[2], two[3], 0x0040), 0x5410);
         *reinterpret_cast<uint32_t *>(rows + kv_place<RB>(t, sub * 4)) = o;
     }
     if (sub == 0) {
-        const uint32_t pair = finite ? sbits | range << 16 : (bf16 ? 0x7fc07fc0u : 0x7e007e00u);
+        const uint32_t pair = finite ? sbits | range << 16 : (BF16 ? 0x7fc07fc0u : 0x7e007e00u);
         *reinterpret_cast<uint32_t *>(granule + kv_param_offset(RB, part) + 4 * t) = pair;
     }
 }
@@ -124,7 +150,7 @@ struct KvWriteArgs {
     int tokens, heads_per_cta;
 };
 
-template <int D, int BITS>
+template <int D, int BITS, bool BF16>
 __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteArgs a)
 {
     constexpr int kLanes = D / 8, kTokens = kKvThreads / kLanes, kGranule = kv_granule_bytes(kv_row_bytes(D, BITS));
@@ -151,25 +177,35 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteArgs 
             ny = *reinterpret_cast<const uint4 *>(vs + (h + 1) * a.v_head_stride);
         }
         uint8_t *granule = kv_granule(a.c, page, place, h, kGranule);
-        quantise_row<D, BITS>(x, sub, place, granule, 0, a.c.bf16, kept);
-        quantise_row<D, BITS>(y, sub, place, granule, 1, a.c.bf16, kept);
+        quantise_row<D, BITS, BF16>(x, sub, place, granule, 0, kept);
+        quantise_row<D, BITS, BF16>(y, sub, place, granule, 1, kept);
         x = nx;
         y = ny;
     }
 }
 
-// eight codes of a row -> eight 16-bit values
-template <int BITS>
-__device__ __forceinline__ uint4 restore8(uint2 codes, float2 p, bool bf16)
+// eight codes of a row -> eight 16-bit values: 0x4b000000 | c is the number 2^23 + c; code * scale is exact in 24 bits, so the multiply-add rounds like the sum
+template <int BITS, bool BF16>
+__device__ __forceinline__ uint4 restore8(uint2 codes, float2 p)
 {
-    float f[8];
+    const uint64_t scale2 = pack_floats(p.x, p.x), min2 = pack_floats(p.y, p.y), off2 = pack_floats(-8388608.f, -8388608.f);
+    uint32_t half[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t c = BITS == 8 ? ((i < 4 ? codes.x : codes.y) >> (8 * (i & 3))) & 255u : (codes.x >> (4 * i)) & 15u;
-        f[i] = fmaf((float)c, p.x, p.y); // one rounding: code * scale is exact in 24 bits, so this is the sum's
+    for (int i = 0; i < 4; ++i) {
+        uint32_t a, b;
+        if (BITS == 8) {
+            const uint32_t w = i < 2 ? codes.x : codes.y;
+            a = __byte_perm(w, 0x4b000000u, (i & 1) ? 0x7442 : 0x7440);
+            b = __byte_perm(w, 0x4b000000u, (i & 1) ? 0x7443 : 0x7441);
+        } else {
+            a = ((codes.x >> (8 * i)) & 15u) | 0x4b000000u;
+            b = ((codes.x >> (8 * i + 4)) & 15u) | 0x4b000000u;
+        }
+        uint32_t lo, hi;
+        unpack_bits(fma_floats(add_floats(pack_floats(__uint_as_float(a), __uint_as_float(b)), off2), scale2, min2), lo, hi);
+        half[i] = float_pair_to_half(__uint_as_float(lo), __uint_as_float(hi), BF16);
     }
-    return make_uint4(float_pair_to_half(f[0], f[1], bf16), float_pair_to_half(f[2], f[3], bf16), float_pair_to_half(f[4], f[5], bf16),
-                      float_pair_to_half(f[6], f[7], bf16));
+    return make_uint4(half[0], half[1], half[2], half[3]);
 }
 
 struct KvReadArgs {
@@ -180,7 +216,7 @@ struct KvReadArgs {
     int rows, batch, table_stride, heads_per_cta;
 };
 
-template <int D, int BITS>
+template <int D, int BITS, bool BF16>
 __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvReadArgs a)
 {
     constexpr int kLanes = D / 8, kTokens = kKvThreads / kLanes, RB = kv_row_bytes(D, BITS), kGranule = kv_granule_bytes(RB);
@@ -226,8 +262,8 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvReadArgs a)
     Item i = load(h0);
     for (int h = h0; h < h1; ++h) {
         const Item next = h + 1 < h1 ? load(h + 1) : i; // under way while this head's values are written
-        *reinterpret_cast<uint4 *>(ko + h * a.k_head_stride) = restore8<BITS>(i.kc, half_pair_to_float(i.kp, a.c.bf16), a.c.bf16);
-        *reinterpret_cast<uint4 *>(vo + h * a.v_head_stride) = restore8<BITS>(i.vc, half_pair_to_float(i.vp, a.c.bf16), a.c.bf16);
+        *reinterpret_cast<uint4 *>(ko + h * a.k_head_stride) = restore8<BITS, BF16>(i.kc, half_pair_to_float(i.kp, BF16));
+        *reinterpret_cast<uint4 *>(vo + h * a.v_head_stride) = restore8<BITS, BF16>(i.vc, half_pair_to_float(i.vp, BF16));
         i = next;
     }
 }
@@ -246,7 +282,7 @@ bool half_rows_valid(const void *p, long long stride, long long head_stride)
 
 static KvShape kv_shape(const abq_kv_cache &c)
 {
-    return { reinterpret_cast<uint8_t *>(c.data), (long long)c.num_pages * c.page_size, c.num_pages, c.page_size, c.kv_heads, c.half_type == ABQ_HALF_BF16 };
+    return { reinterpret_cast<uint8_t *>(c.data), (long long)c.num_pages * c.page_size, c.num_pages, c.page_size, c.kv_heads };
 }
 
 // Heads that a CTA takes one after the other: as many as leave the GPU a few thousand CTAs (a CTA is 16 or 32 tokens), at most 8
@@ -276,6 +312,18 @@ static abq_status launch_kv(Kernel kern, dim3 grid, const Args &args, abq_stream
     return ABQ_OK;
 }
 
+// The kernel's template arguments from a cache's description
+template <typename F>
+static abq_status with_shape(const abq_kv_cache &c, F f)
+{
+    using std::integral_constant;
+    auto typed = [&](auto dim, auto bits) {
+        return c.half_type == ABQ_HALF_BF16 ? f(dim, bits, std::true_type()) : f(dim, bits, std::false_type());
+    };
+    auto sized = [&](auto dim) { return c.bits == 8 ? typed(dim, integral_constant<int, 8>()) : typed(dim, integral_constant<int, 4>()); };
+    return c.head_dim == 128 ? sized(integral_constant<int, 128>()) : sized(integral_constant<int, 64>());
+}
+
 } // namespace abq
 
 extern "C" size_t abq_kv_cache_bytes(const abq_kv_cache *cache)
@@ -299,9 +347,9 @@ extern "C" abq_status abq_kv_cache_write(const abq_kv_write_params *p, abq_strea
     const KvWriteArgs a = { kv_shape(p->cache), reinterpret_cast<const uint8_t *>(p->k), reinterpret_cast<const uint8_t *>(p->v), 2 * p->k_stride,
                             2 * p->k_head_stride, 2 * p->v_stride, 2 * p->v_head_stride, p->slots, p->tokens, hpc };
     const dim3 grid(blocks, (H + hpc - 1) / hpc);
-    if (D == 128)
-        return p->cache.bits == 8 ? launch_kv(kv_write_kernel<128, 8>, grid, a, stream) : launch_kv(kv_write_kernel<128, 4>, grid, a, stream);
-    return p->cache.bits == 8 ? launch_kv(kv_write_kernel<64, 8>, grid, a, stream) : launch_kv(kv_write_kernel<64, 4>, grid, a, stream);
+    return with_shape(p->cache, [&](auto dim, auto bits, auto bf16) {
+        return launch_kv(kv_write_kernel<decltype(dim)::value, decltype(bits)::value, decltype(bf16)::value>, grid, a, stream);
+    });
 }
 
 extern "C" abq_status abq_kv_cache_read(const abq_kv_read_params *p, abq_stream_t stream)
@@ -318,7 +366,7 @@ extern "C" abq_status abq_kv_cache_read(const abq_kv_read_params *p, abq_stream_
     const KvReadArgs a = { kv_shape(p->cache), reinterpret_cast<uint8_t *>(p->k), reinterpret_cast<uint8_t *>(p->v), 2 * p->k_stride, 2 * p->k_head_stride,
                            2 * p->v_stride, 2 * p->v_head_stride, p->block_table, p->cu_seqlens, p->rows, p->batch, p->table_stride, hpc };
     const dim3 grid(blocks, (H + hpc - 1) / hpc);
-    if (D == 128)
-        return p->cache.bits == 8 ? launch_kv(kv_read_kernel<128, 8>, grid, a, stream) : launch_kv(kv_read_kernel<128, 4>, grid, a, stream);
-    return p->cache.bits == 8 ? launch_kv(kv_read_kernel<64, 8>, grid, a, stream) : launch_kv(kv_read_kernel<64, 4>, grid, a, stream);
+    return with_shape(p->cache, [&](auto dim, auto bits, auto bf16) {
+        return launch_kv(kv_read_kernel<decltype(dim)::value, decltype(bits)::value, decltype(bf16)::value>, grid, a, stream);
+    });
 }

@@ -14,12 +14,16 @@
 //   warp 9          issues the products: while one tile's softmax runs, the tensor cores work for the other
 //   warps 10, 11    look through the V tiles that some row of the block does not see to the end: 0 times Inf or NaN is no 0, so such values are set to 0 in
 //                   shared memory and added by the rows that see them when they write their result
-// What bounds it: the tensor cores (4 * 128 * 128 * D operations a tile pair) and, as long for D = 128 and twice as long for D = 64, one exponential per score.
+// What bounds it: the tensor cores (4 * 128 * 128 * D operations a tile pair) and, as long for D = 128 and twice as long for D = 64, one exponential per score on
+// the special-function units.  So part of the exponentials of a tile (kPaPoly of 8 pairs) is computed on the multiply-add pipes, two at a time: 2^x =
+// 2^n 2^f with n = rint(x), a minimax polynomial for 2^f on [-1/2, 1/2] (Remez, relative error 2^-18.5 with five coefficients for fp16, 2^-13.7 with four for
+// bf16), n added to the exponent.  Tiles with masked scores take the units' function for all (it gives the 0 that they need).
 //
 // P is rounded to the 16-bit type (tensor-core operands); fp16 holds p times 2^6, so that weights down to 2^-20 of the maximum keep all bits.  The sum of p is
 // that of the unrounded values.
 #include <cuda.h>
 #include <algorithm>
+#include <type_traits>
 
 #include "abq_kernels.h"
 #include "kv_cache.cuh"
@@ -29,6 +33,7 @@ namespace abq {
 
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128; // keys of a tile
+constexpr int kPaPoly = 3;   // pairs of 8 whose exponentials are polynomials
 
 struct PaArgs {
     const int *cu_q, *cu_k;
@@ -118,7 +123,7 @@ __device__ __forceinline__ float pa_ex2(float x)
 __device__ __forceinline__ float pa_max3(float a, float b, float c)
 {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); // (keeps NaN)
     return r;
 }
 __device__ __forceinline__ uint64_t pa_pack(float lo, float hi)
@@ -139,6 +144,34 @@ __device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c)
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
+}
+
+// 2^x of two numbers of at most 2^14; below 2^-125 it stays there.  NaN is lost: the caller looks for it.
+template <bool BF16>
+__device__ __forceinline__ void pa_ex2_poly(uint64_t x2, float &lo, float &hi)
+{
+    constexpr float kMagic = 12582912.f; // 1.5 * 2^23: the sum's low bits are rint(x)
+    pa_unpack(x2, lo, hi);
+    const uint64_t x = pa_pack(fmaxf(lo, -125.f), fmaxf(hi, -125.f));
+    const uint64_t t = pa_add2(x, pa_pack(kMagic, kMagic));
+    const uint64_t f = pa_add2(x, pa_fma2(t, pa_pack(-1.f, -1.f), pa_pack(kMagic, kMagic)));
+    uint64_t y;
+    auto c = [](float v) { return pa_pack(v, v); };
+    if (BF16) {
+        y = pa_fma2(f, c(0.0551716685295105f), c(0.2426111251115799f));
+        y = pa_fma2(f, y, c(0.6932609677314758f));
+        y = pa_fma2(f, y, c(0.9999280571937561f));
+    } else {
+        y = pa_fma2(f, c(0.009570102207362652f), c(0.05591785907745361f));
+        y = pa_fma2(f, y, c(0.240247443318367f));
+        y = pa_fma2(f, y, c(0.6931217908859253f));
+        y = pa_fma2(f, y, c(0.9999992847442627f));
+    }
+    float n0, n1;
+    pa_unpack(y, lo, hi);
+    pa_unpack(t, n0, n1);
+    lo = __int_as_float(__float_as_int(lo) + (__float_as_int(n0) << 23));
+    hi = __int_as_float(__float_as_int(hi) + (__float_as_int(n1) << 23));
 }
 
 #define PA_REGS32(v)                                                                                                                                       \
@@ -260,7 +293,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 pa_ld_tie(s + 64);
                 pa_ld_tie(s + 96);
                 const int lim = sees - j * kPaKeys;
-                if (__any_sync(0xffffffffu, lim < kPaKeys)) {
+                const bool masked = __any_sync(0xffffffffu, lim < kPaKeys);
+                if (masked) {
 #pragma unroll
                     for (int x = 0; x < 128; ++x)
                         s[x] = x < lim ? s[x] : -INFINITY;
@@ -270,9 +304,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 for (int x = 4; x < 128; x += 8) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        top[e] = x + 4 + e < 128 ? pa_max3(top[e], s[x + e], s[x + 4 + e]) : fmaxf(top[e], s[x + e]);
+                        top[e] = x + 4 + e < 128 ? pa_max3(top[e], s[x + e], s[x + 4 + e]) : pa_max3(top[e], s[x + e], s[x + e]);
                 }
-                const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                const float peak = pa_max3(pa_max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
+                if (!(peak < INFINITY)) // NaN (or an overflow) among the scores: the row's result
+                    l = NAN;
                 const bool raise = peak > m + 8.f;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float f = raise ? pa_ex2(m - peak) : 1.f;
@@ -298,20 +334,31 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 }
                 const float base = (BF16 ? 0.f : 6.f) - (m == -INFINITY ? 0.f : m);
                 const uint64_t scale2 = pa_pack(a.scale_log2, a.scale_log2), base2 = pa_pack(base, base);
+                auto weights = [&](auto poly) {
 #pragma unroll
-                for (int x = 0; x < 128; x += 32) {
-                    uint32_t w[16];
+                    for (int x = 0; x < 128; x += 32) {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float lo, hi;
-                        pa_unpack(pa_fma2(pa_pack(s[x + e], s[x + e + 1]), scale2, base2), lo, hi);
-                        lo = pa_ex2(lo);
-                        hi = pa_ex2(hi);
-                        sum2 = pa_add2(sum2, pa_pack(lo, hi));
-                        w[e >> 1] = float_pair_to_half(lo, hi, BF16);
+                        for (int e = 0; e < 32; e += 2) {
+                            float lo, hi;
+                            const uint64_t y = pa_fma2(pa_pack(s[x + e], s[x + e + 1]), scale2, base2);
+                            if (decltype(poly)::value && (e >> 1) * kPaPoly % 8 < kPaPoly) { // (spread over the 8)
+                                pa_ex2_poly<BF16>(y, lo, hi);
+                            } else {
+                                pa_unpack(y, lo, hi);
+                                lo = pa_ex2(lo);
+                                hi = pa_ex2(hi);
+                            }
+                            sum2 = pa_add2(sum2, pa_pack(lo, hi));
+                            w[e >> 1] = float_pair_to_half(lo, hi, BF16);
+                        }
+                        pa_st16(ts + (x >> 1), w);
                     }
-                    pa_st16(ts + (x >> 1), w);
-                }
+                };
+                if (masked)
+                    weights(std::false_type());
+                else
+                    weights(std::true_type());
                 pa_st_wait();
                 tmem_fence_before();
                 __syncwarp();
@@ -332,7 +379,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 pa_unpack(sum2, lo, hi);
                 l += lo + hi;
                 inv = l == 0.f ? 0.f : 1.f / l;
-                if (it.edge < it.most)
+                if (it.edge < n) // (its tiles have been looked through by now; the other tile's may not)
                     foul = *reinterpret_cast<volatile int *>(&poison[blocks & 3]) | *reinterpret_cast<volatile int *>(&poison[4 + (blocks & 3)]);
             }
             blocks += it.most > 0;
@@ -571,7 +618,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
                 }
                 bad = __any_sync(0xffffffffu, bad);
-                if (j == it.most - 1 && lane == 0)
+                if (lane == 0)
                     poison[4 * half + (blocks & 3)] = bad; // (copies run at most two blocks ahead of the softmax)
                 fence_proxy_async();
                 __syncwarp();

@@ -144,8 +144,8 @@ def prompt_attention(q, k, v, nq, nk, scale):
     """(result, error bound) in float64 of causal attention over packed 16-bit rows (CPU); a value that a row does not see counts as 0.
 
     The bound: the result's rounding and that of p (half a step each; fp16 weights below 2^-20 of the largest lose at most 2^-31 of it per key); the score's
-    error d, at most 2^-20 of scale log2(e) sum|q k| (8 products of 16 in fp32, 2^-23 each), which moves p and the sum of p by at most 2 ln 2 d each; sums in
-    fp32 with the exponential's 2^-22, and O's scaling: 2^-18 of the sum of magnitudes."""
+    error d, at most 2^-20 of scale log2(e) sum|q k| (8 products of 16 in fp32, 2^-23 each), which moves p and the sum of p by at most 2 ln 2 d each; the
+    exponential is off by at most 2^-13.7 (bf16) or 2^-18.5 (fp16), in p and in their sum; sums in fp32 and O's scaling: 2^-18 of the sum of magnitudes."""
     half, heads, H = q.dtype, q.shape[1], k.shape[1]
     step, tiny = halves(half)
     out, bound = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
@@ -158,7 +158,8 @@ def prompt_attention(q, k, v, nq, nk, scale):
             fine = torch.where(vv.isfinite(), vv, torch.zeros_like(vv))
             got = p @ fine
             d = 2.0 ** -20 * 1.4427 * scale * (qq.abs() @ kk.nan_to_num(0.0, 0.0, 0.0).abs().T).amax(-1, keepdim=True)
-            err = (step + 2.78 * d + 2.0 ** -18) * (p @ fine.abs()) + step * got.abs() + tiny + m * 2.0 ** -31 * fine.abs().amax()
+            ex = 2.0 * (2.0 ** -13.7 if half == torch.bfloat16 else 2.0 ** -18.5)
+            err = (step + 2.78 * d + ex + 2.0 ** -18) * (p @ fine.abs()) + step * got.abs() + tiny + m * 2.0 ** -31 * fine.abs().amax()
             hit = seen.double() @ (~vv.isfinite()).double() > 0  # rows that see an Inf or NaN in this feature
             out[a:a + n, h] = torch.where(hit, torch.full_like(got, float("nan")), got)
             bound[a:a + n, h] = err
