@@ -11,7 +11,7 @@
 //   warps 0-3, 4-7  softmax of the two 128-row tiles, a thread per row; they also scale O (only when the maximum has grown by more than 2^8: the
 //                   exponent stays bounded without it) and write the result
 //   warp 8          TMA: Q of a block, K and V tiles in the order of their use through one ring
-//   warp 9          issues the products: while one tile's softmax runs, the tensor cores work for the other
+//   warp 9          issues the products: while one tile's softmax runs, the tensor cores work for the other (D = 64: for the next keys, too)
 //   warps 10, 11    look through the V tiles that some row of the block does not see to the end: 0 times Inf or NaN is no 0, so such values are set to 0 in
 //                   shared memory and added by the rows that see them when they write their result
 // What bounds it: the tensor cores (4 * 128 * 128 * D operations a tile pair) and, as long for D = 128 and twice as long for D = 64, one exponential per score on
@@ -33,7 +33,7 @@ namespace abq {
 
 constexpr int kPaThreads = 384;
 constexpr int kPaKeys = 128; // keys of a tile
-constexpr int kPaPoly = 3;   // pairs of 8 whose exponentials are polynomials
+constexpr int kPaPoly = 1;   // pairs of 8 whose exponentials are polynomials
 
 struct PaArgs {
     const int *cu_q, *cu_k;
@@ -48,9 +48,12 @@ struct PaArgs {
 template <int D>
 struct PaShape {
     static constexpr int kTile = 128 * D * 2, kHalf = 128 * 128, kHalves = D / 64; // a 128-byte-swizzled half holds 64 features
-    static constexpr int kStages = D == 128 ? 5 : 10;
-    static constexpr int kSmem = (2 + kStages) * kTile + 1024 + 512;
-    static constexpr int kO = 256; // TMEM columns: S / P of the tiles at 0 and 128, their O from here
+    // D = 64 leaves TMEM for P beside S, and shared memory for the next block's Q: S of the next keys is made while the softmax of these ones runs
+    static constexpr bool kApart = D == 64;
+    static constexpr int kQBlocks = kApart ? 2 : 1, kStages = kApart ? 9 : 5;
+    static constexpr int kSmem = (2 * kQBlocks + kStages) * kTile + 1024 + 512;
+    // TMEM columns: S of the tiles at 0 and 128, with P over their first half or from 256; then O
+    static constexpr int kP = kApart ? 256 : 0, kPStep = kApart ? 64 : 128, kO = kApart ? 384 : 256;
 };
 
 struct PaItem {
@@ -60,46 +63,82 @@ struct PaItem {
     bool valid;
 };
 
-// Block number `idx`, found by all lanes of a warp: 32 sequences at a time.
-__device__ __forceinline__ PaItem pa_item(const PaArgs &a, int idx, int lane)
+// Rows of sequence b and of its keys, cut to what the arrays hold.
+struct PaSeq {
+    int q0, nq, k0, nk;
+};
+__device__ __forceinline__ PaSeq pa_seq(const PaArgs &a, int b)
+{
+    PaSeq s = { 0, 0, 0, 0 };
+    if (b < a.batch) {
+        s.q0 = min(max(a.cu_q[b], 0), a.total_q);
+        s.nq = min(max(a.cu_q[b + 1], s.q0), a.total_q) - s.q0;
+        s.k0 = min(max(a.cu_k[b], 0), a.total_k);
+        s.nk = min(max(a.cu_k[b + 1], s.k0), a.total_k) - s.k0;
+    }
+    return s;
+}
+__device__ __forceinline__ int pa_scan(int x, int lane) // sum of this and the lanes before
+{
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        x += lane >= o ? y : 0;
+    }
+    return x;
+}
+
+// Block number `idx`, found by all lanes of a warp.  Up to 32 sequences (a lane holds one, `own`): blocks of all sequences by the key tiles they see, most
+// first, so that dealing them to and fro leaves no CTA with much more than the others (16 prompts of 200 to 1023 tokens: 57 tiles on one, 38 on another
+// in the order of the sequences).  More sequences, where chance does that: one after the other, the last block, which sees most, first.
+__device__ __forceinline__ PaItem pa_item(const PaArgs &a, const PaSeq &own, int idx, int lane)
 {
     PaItem it;
-    int slot = idx / a.head_groups;
+    const int shift = 8 - a.pack_log2, tokens = 1 << shift; // of a block
+    int slot = idx / a.head_groups, block = 0, at = 0;
     it.hg = idx - slot * a.head_groups;
     it.valid = false;
-    const int tokens = 256 >> a.pack_log2;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const int b = b0 + lane;
-        int q0 = 0, nq = 0, k0 = 0, nk = 0;
-        if (b < a.batch) {
-            q0 = min(max(a.cu_q[b], 0), a.total_q);
-            nq = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
-            k0 = min(max(a.cu_k[b], 0), a.total_k);
-            nk = min(max(a.cu_k[b + 1], k0), a.total_k) - k0;
+    PaSeq s = own;
+    if (a.batch <= 32) {
+        const int blocks = (s.nq + tokens - 1) >> shift, off = s.nk - s.nq;
+        auto first = [&](int x) { return min(blocks, max(0, (kPaKeys * (x - 1) - off) >> shift)); };                  // block that sees x tiles or more (x > 0)
+        auto count = [&](int x) { return x == 0 ? blocks : s.nk > kPaKeys * (x - 1) ? blocks - first(x) : 0; };       // and how many do
+        int lo = 0, hi = (__reduce_max_sync(0xffffffffu, s.nk) + kPaKeys - 1) / kPaKeys;
+        it.valid = slot < __reduce_add_sync(0xffffffffu, blocks);
+        while (lo < hi) { // the most tiles that more than `slot` blocks see
+            const int mid = (lo + hi + 1) >> 1;
+            if (__reduce_add_sync(0xffffffffu, count(mid)) > slot)
+                lo = mid;
+            else
+                hi = mid - 1;
         }
-        const int blocks = (nq + tokens - 1) / tokens;
-        int end = blocks;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, end, o);
-            end += lane >= o ? x : 0;
+        const int more = count(lo + 1), here = count(lo) - more;
+        slot -= __reduce_add_sync(0xffffffffu, more);
+        const int end = pa_scan(here, lane);
+        at = __ffs(__ballot_sync(0xffffffffu, slot < end)) - 1;
+        block = __shfl_sync(0xffffffffu, (lo ? first(lo) : 0) + slot - (end - here), at & 31);
+    } else {
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            s = pa_seq(a, b0 + lane);
+            const int end = pa_scan((s.nq + tokens - 1) >> shift, lane);
+            const uint32_t behind = __ballot_sync(0xffffffffu, slot < end);
+            if (behind) {
+                at = __ffs(behind) - 1;
+                block = __shfl_sync(0xffffffffu, end, at) - 1 - slot;
+                it.valid = true;
+                break;
+            }
+            slot -= __shfl_sync(0xffffffffu, end, 31);
         }
-        const uint32_t behind = __ballot_sync(0xffffffffu, slot < end);
-        if (behind) {
-            const int at = __ffs(behind) - 1;
-            it.q0 = __shfl_sync(0xffffffffu, q0, at);
-            it.nq = __shfl_sync(0xffffffffu, nq, at);
-            it.k0 = __shfl_sync(0xffffffffu, k0, at);
-            it.nk = __shfl_sync(0xffffffffu, nk, at);
-            it.tok0 = (__shfl_sync(0xffffffffu, end, at) - 1 - slot) * tokens; // the last block, which sees most, first
-            it.off = it.nk - it.nq;
-            it.valid = true;
-            break;
-        }
-        slot -= __shfl_sync(0xffffffffu, end, 31);
     }
     if (!it.valid)
         return it;
+    it.q0 = __shfl_sync(0xffffffffu, s.q0, at);
+    it.nq = __shfl_sync(0xffffffffu, s.nq, at);
+    it.k0 = __shfl_sync(0xffffffffu, s.k0, at);
+    it.nk = __shfl_sync(0xffffffffu, s.nk, at);
+    it.tok0 = block << shift;
+    it.off = it.nk - it.nq;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int first = it.tok0 + t * (tokens >> 1), last = min(it.nq, first + (tokens >> 1)) - 1;
@@ -193,6 +232,15 @@ __device__ __forceinline__ void pa_ld32(uint32_t taddr, float *v)
                  : "r"(taddr));
 }
 __device__ __forceinline__ void pa_ld_wait(float *v) { asm volatile("tcgen05.wait::ld.sync.aligned;" : PA_REGS32(v)::"memory"); }
+__device__ __forceinline__ void pa_ld16(uint32_t taddr, float *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+                   "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void pa_ld_tie(float *v) { asm volatile("" : PA_REGS32(v)); } // (waited for with others)
 __device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t *v)
 {
@@ -202,6 +250,59 @@ __device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t *v)
                  : "memory");
 }
 __device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16-byte pieces w[0..3] of four neighbouring lanes: lane b of them ends with piece b of lane k in w[k]
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4][4], int lane)
+{
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k & o)
+                continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { // keep the piece on the diagonal, trade the other
+                const uint32_t give = up ? w[k][e] : w[k | o][e], got = __shfl_xor_sync(0xffffffffu, give, o);
+                w[k][e] = up ? got : w[k][e];
+                w[k | o][e] = up ? w[k | o][e] : got;
+            }
+        }
+    }
+}
+
+// The rows of a block whose last V tiles held Inf or NaN, once more: the product's part from TMEM, and those values where a row sees them (they were left out of
+// the product).  Rare, and apart so that the usual path stays short.
+template <int D, bool BF16>
+__device__ __noinline__ void add_foul_values(const PaArgs &a, uint32_t to, int q_row, bool live, int head, int k0, int first, int sees, float inv)
+{
+    const uint8_t *v = a.v + (long long)k0 * a.v_stride + (long long)(head / a.group) * a.v_head_stride;
+    uint8_t *dst = a.out + (long long)q_row * a.out_stride + (long long)head * a.out_head_stride;
+#pragma unroll 1
+    for (int x = 0; x < D; x += 16) {
+        float o[16];
+        pa_ld16(to + x, o);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            o[e] *= inv;
+        for (int k = first; k < sees; ++k) {
+            const unsigned short *vr = reinterpret_cast<const unsigned short *>(v + (long long)k * a.v_stride) + x;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float f = half_bits_to_float(vr[e], BF16);
+                if (!(fabsf(f) <= 3.402823466e38f))
+                    o[e] += f;
+            }
+        }
+        if (live) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+                *reinterpret_cast<uint4 *>(dst + 2 * (x + e)) =
+                    make_uint4(float_pair_to_half(o[e], o[e + 1], BF16), float_pair_to_half(o[e + 2], o[e + 3], BF16),
+                               float_pair_to_half(o[e + 4], o[e + 5], BF16), float_pair_to_half(o[e + 6], o[e + 7], BF16));
+        }
+    }
+}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPaThreads, 1)
@@ -215,21 +316,29 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     constexpr uint32_t kIdescO = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint8_t *sq = smem, *ring = smem + 2 * kTile;
+    constexpr bool kApart = Sh::kApart;
+    constexpr int kQBlocks = Sh::kQBlocks;
+    uint8_t *sq = smem, *ring = smem + 2 * kQBlocks * kTile;
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + kStages * kTile);
-    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *p_ready = bars + 4, *drain = bars + 6;
-    uint64_t *kv_full = bars + 8, *kv_empty = kv_full + kStages, *edge_full = kv_empty + kStages;
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *s_read = bars + 8, *o_done = bars + 10, *drain = bars + 12, *half_way = bars + 13;
+    uint64_t *kv_full = bars + 15, *kv_empty = kv_full + kStages, *edge_full = kv_empty + kStages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(edge_full + kStages);
     int *poison = reinterpret_cast<int *>(tmem_slot + 2); // [2 warps][4 blocks]: V tiles of the block held Inf or NaN
 
+    // No barrier completes a phase before everybody who waits for the one before has seen that: a parity that is asked for two phases late looks like one
+    // that has not come.  s_full: the scores of the next keys follow p_ready (or s_read), which follows the wait for these.  o_done: the next product it
+    // stands for follows a p_ready behind the wait.  p_ready and s_read: their next arrival follows an s_full that the MMA warp sends after its wait.
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
         mbar_init(drain, 1);
         for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 1);
+            mbar_init(&q_empty[t], 1);
             mbar_init(&s_full[t], 1);
             mbar_init(&p_ready[t], 4);
+            mbar_init(&s_read[t], 4);
+            mbar_init(&o_done[t], 1);
+            mbar_init(&half_way[t], 4);
         }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&kv_full[s], 2); // the producer twice, or the two warps that looked through the tile
@@ -253,6 +362,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     pdl_wait_prior_grid();
 
     // The pool is what the block was launched with: 384 threads x 168 registers = 256 x 208 + 128 x 88
+    const PaSeq own = pa_seq(a, a.batch <= 32 ? lane : a.batch);
     const int G = gridDim.x, c = blockIdx.x;
     auto number = [&](int round) { return round * G + (round & 1 ? G - 1 - c : c); };
 
@@ -263,16 +373,17 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + (uint32_t)(t * 128), to = tmem + lanes + (uint32_t)(Sh::kO + t * D);
+        const uint32_t ts = tmem + lanes + (uint32_t)(t * 128), tp = tmem + lanes + (uint32_t)(Sh::kP + t * Sh::kPStep), to = tmem + lanes + (uint32_t)(Sh::kO + t * D);
         const int pack = 1 << a.pack_log2;
-        uint32_t phase = 0;
-        int blocks = 0; // with a key
+        uint32_t phase = 0, done = 0, others = 0; // of s_full; of o_done (a product with V each, or with S and P in one place a block); key tiles of the other row tile so far
+        int blocks = 0;               // with a key
         bool ok = true;
+        PaItem next = pa_item(a, own, number(0), lane);
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, number(round), lane);
+            const PaItem it = next;
             if (!it.valid)
                 break;
-            const int token = it.tok0 + t * (128 >> a.pack_log2) + (row >> a.pack_log2), head = it.hg * pack + (row & (pack - 1));
+            const int token = it.tok0 + t * (128 >> a.pack_log2) + (row >> a.pack_log2);
             const int sees = min(it.nk, token + it.off + 1);
             float m = -INFINITY;
             uint64_t sum2 = 0;
@@ -292,6 +403,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 pa_ld_tie(s + 32);
                 pa_ld_tie(s + 64);
                 pa_ld_tie(s + 96);
+                if (kApart) { // these scores are in registers: their columns may take the next ones
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&s_read[t]);
+                }
                 const int lim = sees - j * kPaKeys;
                 const bool masked = __any_sync(0xffffffffu, lim < kPaKeys);
                 if (masked) {
@@ -309,6 +426,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 const float peak = pa_max3(pa_max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
                 if (!(peak < INFINITY)) // NaN (or an overflow) among the scores: the row's result
                     l = NAN;
+                if (kApart && j > 0) { // the product with the P before: its columns and O are free
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[t], (done + j - 1) & 1, a.status, STATUS_TIMEOUT_MMA));
+                    if (!ok)
+                        break;
+                    tmem_fence_after();
+                }
                 const bool raise = peak > m + 8.f;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float f = raise ? pa_ex2(m - peak) : 1.f;
@@ -334,6 +457,18 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 }
                 const float base = (BF16 ? 0.f : 6.f) - (m == -INFINITY ? 0.f : m);
                 const uint64_t scale2 = pa_pack(a.scale_log2, a.scale_log2), base2 = pa_pack(base, base);
+                // D = 64: the two tiles' softmaxes would fall into step and take turns at leaving the special-function units idle and fighting for them.  Each starts its
+                // exponentials when the other is half way through its own: tile 0 after tile 1's of the keys before, tile 1 after tile 0's of the same
+                // keys.  Only a matter of time: nothing depends on it, and the wait is given up after a few microseconds.
+                if (kApart) {
+                    const int theirs = t ? j : j - 1;
+                    if (theirs >= 0 && theirs < (t ? it.n[0] : it.n[1])) {
+#pragma unroll 1
+                        for (int i = 0; i < 64 && !mbar_try_wait(&half_way[t ^ 1], (others + theirs) & 1); ++i)
+                            ;
+                        __syncwarp();
+                    }
+                }
                 auto weights = [&](auto poly) {
 #pragma unroll
                     for (int x = 0; x < 128; x += 32) {
@@ -341,18 +476,21 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             float lo, hi;
-                            const uint64_t y = pa_fma2(pa_pack(s[x + e], s[x + e + 1]), scale2, base2);
                             if (decltype(poly)::value && (e >> 1) * kPaPoly % 8 < kPaPoly) { // (spread over the 8)
-                                pa_ex2_poly<BF16>(y, lo, hi);
+                                pa_ex2_poly<BF16>(pa_fma2(pa_pack(s[x + e], s[x + e + 1]), scale2, base2), lo, hi);
                             } else {
-                                pa_unpack(y, lo, hi);
-                                lo = pa_ex2(lo);
-                                hi = pa_ex2(hi);
+                                lo = pa_ex2(fmaf(s[x + e], a.scale_log2, base));
+                                hi = pa_ex2(fmaf(s[x + e + 1], a.scale_log2, base));
                             }
                             sum2 = pa_add2(sum2, pa_pack(lo, hi));
                             w[e >> 1] = float_pair_to_half(lo, hi, BF16);
                         }
-                        pa_st16(ts + (x >> 1), w);
+                        pa_st16(tp + (x >> 1), w);
+                        if (kApart && x == 32) {
+                            __syncwarp();
+                            if (lane == 0)
+                                mbar_arrive(&half_way[t]);
+                        }
                     }
                 };
                 if (masked)
@@ -367,13 +505,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             if (!ok)
                 break;
+            next = pa_item(a, own, number(round + 1), lane); // (while the last product runs)
             float inv = 0.f;
             bool foul = false;
             if (n > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[t], phase & 1, a.status, STATUS_TIMEOUT_MMA));
+                done += kApart ? n : 1;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[t], (done - 1) & 1, a.status, STATUS_TIMEOUT_MMA));
                 if (!ok)
                     break;
-                ++phase;
                 tmem_fence_after();
                 float lo, hi;
                 pa_unpack(sum2, lo, hi);
@@ -383,8 +522,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     foul = *reinterpret_cast<volatile int *>(&poison[blocks & 3]) | *reinterpret_cast<volatile int *>(&poison[4 + (blocks & 3)]);
             }
             blocks += it.most > 0;
-            uint8_t *dst = a.out + (long long)(it.q0 + token) * a.out_stride + (long long)head * a.out_head_stride;
-            const int kv_head = (it.hg << a.pack_log2) / a.group;
+            others += t ? it.n[0] : it.n[1];
+            // Four lanes exchange their 16-byte pieces, so that a store covers 64 bytes of 8 rows and not 16 of 32: lane 4 a + b gets piece b of rows 4 a ..
+            uint8_t *dst[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r2 = (row & ~3) + k, token2 = it.tok0 + t * (128 >> a.pack_log2) + (r2 >> a.pack_log2);
+                dst[k] = token2 >= it.nq ? nullptr
+                                         : a.out + (long long)(it.q0 + token2) * a.out_stride + (long long)(it.hg * pack + (r2 & (pack - 1))) * a.out_head_stride + (lane & 3) * 16;
+            }
 #pragma unroll 1
             for (int x = 0; x < D; x += 32) {
                 float o[32];
@@ -396,27 +542,19 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     for (int e = 0; e < 32; ++e)
                         o[e] = 0.f;
                 }
+                uint32_t w[4][4];
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    o[e] = l == 0.f ? 0.f : o[e] * inv;
-                if (foul) { // Inf and NaN among the values that this row sees in the last tiles (they were left out of the product)
-                    for (int k = it.edge * kPaKeys; k < sees; ++k) {
-                        const unsigned short *vr = reinterpret_cast<const unsigned short *>(a.v + (long long)(it.k0 + k) * a.v_stride + (long long)kv_head * a.v_head_stride) + x;
+                for (int e = 0; e < 32; e += 2) // (a row that saw nothing: P and O are 0)
+                    w[e >> 3][(e >> 1) & 3] = float_pair_to_half(o[e] * inv, o[e + 1] * inv, BF16);
+                transpose4(w, lane);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float f = half_bits_to_float(vr[e], BF16);
-                            if (!(fabsf(f) <= 3.402823466e38f))
-                                o[e] += f;
-                        }
-                    }
-                }
-                if (token < it.nq) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4 *>(dst + 2 * (x + e)) =
-                            make_uint4(float_pair_to_half(o[e], o[e + 1], BF16), float_pair_to_half(o[e + 2], o[e + 3], BF16),
-                                       float_pair_to_half(o[e + 4], o[e + 5], BF16), float_pair_to_half(o[e + 6], o[e + 7], BF16));
-                }
+                for (int k = 0; k < 4; ++k)
+                    if (dst[k])
+                        *reinterpret_cast<uint4 *>(dst[k] + 2 * x) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+            }
+            if (foul) { // (the same for the whole warp)
+                __syncwarp(); // what other lanes have written of this row comes first
+                add_foul_values<D, BF16>(a, to, it.q0 + token, token < it.nq, it.hg * pack + (row & (pack - 1)), it.k0, it.edge * kPaKeys, sees, inv);
             }
             tmem_fence_before(); // (O is read before the next block's first product, which waits for this tile's p)
         }
@@ -426,7 +564,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t edges = 0, last_edge = 0;                 // a bit per stage: parity of edge_full; whether the last tile went there
         bool ok = true;
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, number(round), lane);
+            const PaItem it = pa_item(a, own, number(round), lane);
             if (!it.valid)
                 break;
             if (it.most == 0)
@@ -436,18 +574,19 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             if (elect_one()) {
                 leader = true;
                 for (int i = 0; i < total; ++i) {
-                    if (i == 1) { // Q behind the first K tile: its place is free when the last block's S are done
-                        if (blocks && !mbar_wait_bounded(q_empty, (blocks - 1) & 1, a.status, STATUS_TIMEOUT_PIPE)) {
+                    if (i == 1) { // Q behind the first K tile: its place is free when the S of the block before (or the one before that) are done
+                        const int qb = blocks % kQBlocks, use = blocks / kQBlocks;
+                        if (use && !mbar_wait_bounded(&q_empty[qb], (use - 1) & 1, a.status, STATUS_TIMEOUT_PIPE)) {
                             fine = false;
                             break;
                         }
-                        mbar_arrive_expect_tx(q_full, (uint32_t)kTile * ((it.n[0] > 0) + (it.n[1] > 0)));
+                        mbar_arrive_expect_tx(&q_full[qb], (uint32_t)kTile * ((it.n[0] > 0) + (it.n[1] > 0)));
                         ++queries;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
                             if (it.n[t] > 0)
                                 for (int h = 0; h < kHalves; ++h)
-                                    tma_load_3d(sq + t * kTile + h * kHalf, &tmap_q, h * 128, it.hg * pack, it.q0 + it.tok0 + t * (128 >> a.pack_log2), q_full);
+                                    tma_load_3d(sq + (2 * qb + t) * kTile + h * kHalf, &tmap_q, h * 128, it.hg * pack, it.q0 + it.tok0 + t * (128 >> a.pack_log2), &q_full[qb]);
                     }
                     const int at = place + i, s = at % kStages;
                     if (at >= kStages && !mbar_wait_bounded(&kv_empty[s], ((at / kStages) - 1) & 1, a.status, STATUS_TIMEOUT_PIPE)) {
@@ -489,8 +628,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 else
                     mbar_wait_bounded(&kv_full[s], (at / kStages) & 1, a.status, STATUS_TIMEOUT_TMA);
             }
-            if (queries)
-                mbar_wait_bounded(q_full, (queries - 1) & 1, a.status, STATUS_TIMEOUT_TMA);
+            for (int q = max(0, queries - kQBlocks); q < queries; ++q)
+                mbar_wait_bounded(&q_full[q % kQBlocks], (q / kQBlocks) & 1, a.status, STATUS_TIMEOUT_TMA);
         }
     } else if (warp == 9) {
         // ---------------------------------------------------------------- products
@@ -498,7 +637,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t p_phase[2] = { 0, 0 };
         bool ok = true;
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, number(round), lane);
+            const PaItem it = pa_item(a, own, number(round), lane);
             if (!it.valid)
                 break;
             if (it.most == 0)
@@ -506,8 +645,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             bool fine = true;
             if (elect_one()) {
                 auto wait_kv = [&](int at) { return mbar_wait_bounded(&kv_full[at % kStages], (at / kStages) & 1, a.status, STATUS_TIMEOUT_TMA); };
+                const int qb = blocks % kQBlocks;
                 auto scores = [&](int t, int at) {
-                    const uint32_t qa = smem_u32(sq + t * kTile), ka = smem_u32(ring + (at % kStages) * kTile);
+                    const uint32_t qa = smem_u32(sq + (2 * qb + t) * kTile), ka = smem_u32(ring + (at % kStages) * kTile);
 #pragma unroll
                     for (int h = 0; h < kHalves; ++h) {
                         const uint64_t dq = make_smem_desc_sw128(qa + h * kHalf), dk = make_smem_desc_sw128(ka + h * kHalf);
@@ -517,19 +657,62 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
                     umma_commit(&s_full[t]);
                 };
-                fine = mbar_wait_bounded(q_full, blocks & 1, a.status, STATUS_TIMEOUT_TMA) && wait_kv(place);
+                auto values = [&](int t, int j, int at) {
+                    const uint64_t dv = make_smem_desc_sw128_mn(smem_u32(ring + (at % kStages) * kTile), kHalf);
+#pragma unroll
+                    for (int x = 0; x < kPaKeys / 16; ++x) // 16 keys a step: 16 rows of V, 8 columns of P
+                        umma_f16_ts(tmem + (uint32_t)(Sh::kO + t * D), tmem + (uint32_t)(Sh::kP + t * Sh::kPStep + 8 * x), dv + (uint64_t)(x * 2048 >> 4), kIdescO, (j | x) != 0);
+                };
+                // scores of key tile j; where P lies beside S they only wait until the softmax has read those before them
+                auto free_scores = [&](int t, int j) {
+                    const uint32_t before = p_phase[t] + j; // tiles of scores so far
+                    return !kApart || before == 0 || mbar_wait_bounded(&s_read[t], (before - 1) & 1, a.status, STATUS_TIMEOUT_PIPE);
+                };
+                fine = mbar_wait_bounded(&q_full[qb], (blocks / kQBlocks) & 1, a.status, STATUS_TIMEOUT_TMA) && wait_kv(place);
                 if (fine) {
-                    tmem_fence_after();
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
-                        if (it.n[t] > 0)
-                            scores(t, place);
+                        if (it.n[t] > 0 && fine) {
+                            fine = free_scores(t, 0);
+                            tmem_fence_after();
+                            if (fine)
+                                scores(t, place);
+                        }
                     umma_commit(&kv_empty[place % kStages]);
                     if (it.most == 1)
-                        umma_commit(q_empty);
+                        umma_commit(&q_empty[qb]);
                 }
                 for (int j = 0; j < it.most && fine; ++j) {
                     const int vat = place + pa_v_place(j, it.most), kat = place + pa_k_place(j + 1);
+                    if (kApart) {
+                        if (j + 1 < it.most) {
+                            fine = wait_kv(kat);
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                if (j + 1 < it.n[t] && fine) {
+                                    fine = free_scores(t, j + 1);
+                                    tmem_fence_after();
+                                    if (fine)
+                                        scores(t, kat);
+                                }
+                            umma_commit(&kv_empty[kat % kStages]);
+                            if (j + 2 == it.most)
+                                umma_commit(&q_empty[qb]);
+                        }
+                        fine = fine && wait_kv(vat);
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            if (j < it.n[t] && fine) {
+                                fine = mbar_wait_bounded(&p_ready[t], (p_phase[t] + j) & 1, a.status, STATUS_TIMEOUT_PIPE);
+                                tmem_fence_after();
+                                if (fine) {
+                                    values(t, j, vat);
+                                    umma_commit(&o_done[t]);
+                                }
+                            }
+                        umma_commit(&kv_empty[vat % kStages]);
+                        continue;
+                    }
                     bool have_v = false, have_k = false;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -540,12 +723,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                             continue;
                         have_v = true;
                         tmem_fence_after();
-                        const uint64_t dv = make_smem_desc_sw128_mn(smem_u32(ring + (vat % kStages) * kTile), kHalf);
-#pragma unroll
-                        for (int x = 0; x < kPaKeys / 16; ++x) // 16 keys a step: 16 rows of V, 8 columns of P
-                            umma_f16_ts(tmem + (uint32_t)(Sh::kO + t * D), tmem + (uint32_t)(t * 128 + 8 * x), dv + (uint64_t)(x * 2048 >> 4), kIdescO, (j | x) != 0);
+                        values(t, j, vat);
                         if (j == it.n[t] - 1) {
-                            umma_commit(&s_full[t]); // O is complete
+                            umma_commit(&o_done[t]); // O is complete (a barrier of its own: the next block's scores may be done before anybody has looked)
                         } else {
                             fine = have_k || wait_kv(kat);
                             if (!fine)
@@ -559,7 +739,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     if (j + 1 < it.most)
                         umma_commit(&kv_empty[kat % kStages]);
                     if (j + 2 == it.most)
-                        umma_commit(q_empty);
+                        umma_commit(&q_empty[qb]);
                 }
             }
             __syncwarp();
@@ -581,7 +761,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t edges = 0;
         bool ok = true;
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, number(round), lane);
+            const PaItem it = pa_item(a, own, number(round), lane);
             if (!it.valid)
                 break;
             if (it.most == 0)
