@@ -41,6 +41,7 @@ struct PaArgs {
     uint8_t *out;
     long long v_stride, v_head_stride, out_stride, out_head_stride; // bytes
     int total_q, total_k, batch, head_groups, pack_log2, group;
+    int sorted; // blocks by the key tiles they see (several rounds of blocks, 2 to 32 sequences)
     float scale_log2;
     int *status;
 };
@@ -88,18 +89,19 @@ __device__ __forceinline__ int pa_scan(int x, int lane) // sum of this and the l
     return x;
 }
 
-// Block number `idx`, found by all lanes of a warp.  Up to 32 sequences (a lane holds one, `own`): blocks of all sequences by the key tiles they see, most
-// first, so that dealing them to and fro leaves no CTA with much more than the others (16 prompts of 200 to 1023 tokens: 57 tiles on one, 38 on another
-// in the order of the sequences).  More sequences, where chance does that: one after the other, the last block, which sees most, first.
-__device__ __forceinline__ PaItem pa_item(const PaArgs &a, const PaSeq &own, int idx, int lane)
+// Block number `idx`, found by all lanes of a warp.  Sorted (up to 32 sequences, a lane looks at one): blocks of all sequences by the key tiles they see,
+// most first, so that dealing them to and fro leaves no CTA with much more than the others (16 prompts of 200 to 1023 tokens: 57 tiles on one, 38 on another
+// in the order of the sequences).  Otherwise one sequence after the other, the last block, which sees most, first.
+__device__ __forceinline__ PaItem pa_item(const PaArgs &a, int idx, int lane)
 {
     PaItem it;
     const int shift = 8 - a.pack_log2, tokens = 1 << shift; // of a block
     int slot = idx / a.head_groups, block = 0, at = 0;
     it.hg = idx - slot * a.head_groups;
     it.valid = false;
-    PaSeq s = own;
-    if (a.batch <= 32) {
+    PaSeq s;
+    if (a.sorted) {
+        s = pa_seq(a, lane);
         const int blocks = (s.nq + tokens - 1) >> shift, off = s.nk - s.nq;
         auto first = [&](int x) { return min(blocks, max(0, (kPaKeys * (x - 1) - off) >> shift)); };                  // block that sees x tiles or more (x > 0)
         auto count = [&](int x) { return x == 0 ? blocks : s.nk > kPaKeys * (x - 1) ? blocks - first(x) : 0; };       // and how many do
@@ -362,7 +364,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     pdl_wait_prior_grid();
 
     // The pool is what the block was launched with: 384 threads x 168 registers = 256 x 208 + 128 x 88
-    const PaSeq own = pa_seq(a, a.batch <= 32 ? lane : a.batch);
     const int G = gridDim.x, c = blockIdx.x;
     auto number = [&](int round) { return round * G + (round & 1 ? G - 1 - c : c); };
 
@@ -378,7 +379,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t phase = 0, done = 0, others = 0; // of s_full; of o_done (a product with V each, or with S and P in one place a block); key tiles of the other row tile so far
         int blocks = 0;               // with a key
         bool ok = true;
-        PaItem next = pa_item(a, own, number(0), lane);
+        PaItem next = pa_item(a, number(0), lane);
         for (int round = 0; ok; ++round) {
             const PaItem it = next;
             if (!it.valid)
@@ -505,7 +506,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             }
             if (!ok)
                 break;
-            next = pa_item(a, own, number(round + 1), lane); // (while the last product runs)
+            next = pa_item(a, number(round + 1), lane); // (while the last product runs)
             float inv = 0.f;
             bool foul = false;
             if (n > 0) {
@@ -564,7 +565,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t edges = 0, last_edge = 0;                 // a bit per stage: parity of edge_full; whether the last tile went there
         bool ok = true;
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, own, number(round), lane);
+            const PaItem it = pa_item(a, number(round), lane);
             if (!it.valid)
                 break;
             if (it.most == 0)
@@ -637,7 +638,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t p_phase[2] = { 0, 0 };
         bool ok = true;
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, own, number(round), lane);
+            const PaItem it = pa_item(a, number(round), lane);
             if (!it.valid)
                 break;
             if (it.most == 0)
@@ -761,7 +762,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         uint32_t edges = 0;
         bool ok = true;
         for (int round = 0; ok; ++round) {
-            const PaItem it = pa_item(a, own, number(round), lane);
+            const PaItem it = pa_item(a, number(round), lane);
             if (!it.valid)
                 break;
             if (it.most == 0)
@@ -899,6 +900,7 @@ extern "C" abq_status abq_prompt_attention(const abq_prompt_attention_params *p,
     a.v_stride = 2 * p->v_stride, a.v_head_stride = 2 * p->v_head_stride, a.out_stride = 2 * p->out_stride, a.out_head_stride = 2 * p->out_head_stride;
     a.total_q = p->total_q, a.total_k = p->total_k, a.batch = p->batch, a.head_groups = (int)head_groups, a.pack_log2 = pl, a.group = group;
     a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.sorted = p->batch > 1 && p->batch <= 32 && slots * head_groups > 148;
     a.status = p->status_word;
     const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(148, slots * head_groups));
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
