@@ -9,10 +9,10 @@ template <int NT>
 cudaError_t launch_cache_attention(const CacheAttnArgs &args, int head_dim, int bits, bool bf16, cudaStream_t stream);
 extern template cudaError_t launch_cache_attention<1>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
 extern template cudaError_t launch_cache_attention<2>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
-extern template cudaError_t launch_cache_attention<4>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
 
-// Tiles of 8 query rows that a block holds: one conversion of the codes serves them all; 32 rows are what the registers hold.
-static int row_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+// Tiles of 8 query rows that a block holds.  One conversion of the codes serves them all, but with more rows fewer warps fit: blocks of 16 measured faster than
+// of 32 for 26 rows over 40 heads of 128, 8 bits (36.8 and 43.5 us; blocks of 8: 41.8), and nearly as fast for 256 rows of 64, 4 bits (57.4 and 53.7).
+static int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
 static int most_runs(int tiles) { return kCaSms * ca_ctas_per_sm(tiles) * kCaWarps; }
 
@@ -59,6 +59,7 @@ extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, a
     a.num_pages = p->cache.num_pages, a.page_granules = p->cache.page_size / 16, a.kv_heads = p->cache.kv_heads, a.batch = p->batch, a.n = p->rows_per_seq;
     a.group = p->q_heads / p->cache.kv_heads, a.table_stride = p->table_stride;
     a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.page_magic = ((1ull << 34) + a.page_granules - 1) / a.page_granules;
     const int rows = a.n * a.group, tiles = row_tiles(rows);
     a.row_blocks = (rows + 8 * tiles - 1) / (8 * tiles);
     a.slot_rows = std::min(rows, 8 * tiles);
@@ -68,9 +69,7 @@ extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, a
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int D = p->cache.head_dim, bits = p->cache.bits;
     const bool bf16 = p->cache.half_type == ABQ_HALF_BF16;
-    const cudaError_t e = tiles == 1   ? launch_cache_attention<1>(a, D, bits, bf16, s)
-                          : tiles == 2 ? launch_cache_attention<2>(a, D, bits, bf16, s)
-                                       : launch_cache_attention<4>(a, D, bits, bf16, s);
+    const cudaError_t e = tiles == 1 ? launch_cache_attention<1>(a, D, bits, bf16, s) : launch_cache_attention<2>(a, D, bits, bf16, s);
     if (e != cudaSuccess) {
         set_last_cuda_error(e);
         return ABQ_ERR_CUDA;

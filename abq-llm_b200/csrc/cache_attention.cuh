@@ -46,6 +46,7 @@ struct CacheAttnArgs {
     int *status;
     int num_pages, page_granules, kv_heads, batch, n, group, row_blocks, slot_rows, table_stride, runs;
     float scale_log2;
+    unsigned long long page_magic;
 };
 
 __device__ __forceinline__ int ca_tokens(const CacheAttnArgs &a, int b)
@@ -74,7 +75,14 @@ __device__ __forceinline__ void ca_sums(const CacheAttnArgs &a, int before, long
     all = s;
     prefix = p;
 }
-__device__ __forceinline__ long long ca_quota(const CacheAttnArgs &a, long long total) { return max((total + a.runs - 1) / a.runs, (long long)kCaMinQuota); }
+// Quotient of numbers that hardly ever need 64 bits (their division is some ten times slower)
+__device__ __forceinline__ long long ca_div(long long x, long long y)
+{
+    return ((unsigned long long)(x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
+}
+__device__ __forceinline__ long long ca_quota(const CacheAttnArgs &a, long long total) { return max(ca_div(total + a.runs - 1, a.runs), (long long)kCaMinQuota); }
+// Entry of a block table that holds granule g (page_magic = ceil(2^34 / page_granules): exact for granule numbers below 2^28)
+__device__ __forceinline__ int ca_entry(const CacheAttnArgs &a, int g) { return (int)(((unsigned long long)(uint32_t)g * a.page_magic) >> 34); }
 
 __device__ __forceinline__ float ex2(float x)
 {
@@ -132,8 +140,7 @@ __device__ __forceinline__ void lds(uint32_t *dst, const uint8_t *src)
 template <int D, int BITS, int NT>
 struct CaShape {
     static constexpr int RB = kv_row_bytes(D, BITS), kGranule = kv_granule_bytes(RB), kRows = 8 * NT, kSteps = D / 16;
-    static constexpr bool kQRegs = NT <= 2; // otherwise the fragments wait in shared memory
-    static constexpr int kFixed = kCaWarps * ((kQRegs ? 0 : NT * kSteps * 32 * 8) + kRows * 8);
+    static constexpr int kFixed = kCaWarps * kRows * 8;
     static constexpr int kRoom = 226 * 1024 / ca_ctas_per_sm(NT) - 1024 - kFixed;
     static constexpr int kFit = kRoom / (kCaWarps * (kGranule + 8));
     static constexpr int kStages = kFit < 10 ? kFit : 10;
@@ -150,12 +157,10 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
     constexpr float kCentre = (float)(1 << (BITS - 1));
     constexpr float kKeyScale = BITS == 8 ? 1.f : 64.f, kKeyOffset = BITS == 8 ? -1024.f : -64.f; // code = factor * kKeyScale + kKeyOffset
     constexpr bool kRemainder = NT == 1 && !BF16;
-    constexpr bool kQRegs = Sh::kQRegs;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
     uint8_t *ring = smem + warp * kStages * kGranule;
-    uint2 *qfrag = reinterpret_cast<uint2 *>(smem + kCaWarps * kStages * kGranule) + (kQRegs ? 0 : warp * NT * kSteps * 32);
-    uint64_t *masks = reinterpret_cast<uint64_t *>(reinterpret_cast<uint2 *>(smem + kCaWarps * kStages * kGranule) + (kQRegs ? 0 : kCaWarps * NT * kSteps * 32)) + warp * kRows;
+    uint64_t *masks = reinterpret_cast<uint64_t *>(smem + kCaWarps * kStages * kGranule) + warp * kRows;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + kCaWarps * kStages * kGranule + Sh::kFixed) + warp * kStages;
     if (lane < kStages)
         mbar_init(&full[lane], 1);
@@ -166,36 +171,43 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
 
     // ---- this warp's run of the line
     const int items = a.kv_heads * a.row_blocks, run = blockIdx.x * kCaWarps + warp;
-    long long units, unused;
-    ca_sums(a, 0, units, unused);
-    units *= items;
-    const long long quota = ca_quota(a, units);
-    long long left = min(units, (run + 1) * quota) - run * quota;
-    if (left <= 0)
-        return; // (before any copy)
     int b = 0, G = 0, item, pos;
+    long long left;
     {
-        long long rem = run * quota; // from the start of sequence b
+        long long units = 0, quota = 0, rem = 0, unused;
+        if (a.batch > 32) {
+            ca_sums(a, 0, units, unused);
+            quota = ca_quota(a, units * items);
+        }
         for (int b0 = 0;; b0 += 32) { // 32 sequences at a time
             const int own = b0 + lane < a.batch ? ca_granules(a, b0 + lane) : 0;
-            long long end = ca_units(own);
+            uint32_t upto = ca_units(own);
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, end, o);
-                end += lane >= o ? x : 0;
+                const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+                upto += lane >= o ? x : 0;
             }
-            end *= items;
-            const uint32_t behind = __ballot_sync(0xffffffffu, rem < end);
+            if (b0 == 0) {
+                if (a.batch <= 32) {
+                    units = __shfl_sync(0xffffffffu, upto, 31);
+                    quota = ca_quota(a, units * items);
+                }
+                rem = run * quota; // from the start of sequence b0
+                left = min(units * items, rem + quota) - rem;
+                if (left <= 0)
+                    return; // (before any copy)
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, rem < (long long)upto * items);
             if (behind) {
                 const int at = __ffs(behind) - 1;
                 b = b0 + at;
                 G = __shfl_sync(0xffffffffu, own, at);
-                rem -= __shfl_sync(0xffffffffu, end, at) - (long long)ca_units(G) * items;
+                rem -= (long long)(__shfl_sync(0xffffffffu, upto, at) - ca_units(G)) * items;
                 break;
             }
-            rem -= __shfl_sync(0xffffffffu, end, 31);
+            rem -= (long long)__shfl_sync(0xffffffffu, upto, 31) * items;
         }
-        item = (int)(rem / ca_units(G));
+        item = (int)ca_div(rem, ca_units(G));
         pos = (int)(rem - (long long)item * ca_units(G));
     }
 
@@ -213,7 +225,7 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
         const int g = p.g0 + base + lane;
         t.at = ~0u;
         if (g < p.g1) {
-            const int entry = g / a.page_granules, page = a.table[(size_t)p.b * a.table_stride + entry];
+            const int entry = ca_entry(a, g), page = a.table[(size_t)p.b * a.table_stride + entry];
             if (page >= 0 && page < a.num_pages)
                 t.at = ((uint32_t)page * a.kv_heads + p.item / a.row_blocks) * a.page_granules + (g - entry * a.page_granules);
             else if (a.status)
@@ -261,22 +273,39 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
         return false;
     };
 
+    const int rows = a.n * a.group;
+    // the 16 bytes x of this lane's queries in tile t of an item
+    auto query = [&](const Piece &p, int t, int x) -> const uint8_t * {
+        const int head = p.item / a.row_blocks, at = (p.item - head * a.row_blocks) * kRows + 8 * t + r, i = at / a.group;
+        // 8 bits: features 16 q .. of each 64; 4 bits: a quarter of the row
+        const int byte = BITS == 8 ? (x >> 1) * 128 + q * 32 + (x & 1) * 16 : q * (D / 2) + x * 16;
+        return at < rows ? a.q + ((long long)p.b * a.n + i) * a.q_stride + (long long)(head * a.group + at - i * a.group) * a.q_head_stride + byte : nullptr;
+    };
+    auto prefetch_queries = [&](const Piece &p) { // (they are used behind the first copies, which need the block table first)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (const uint8_t *at = query(p, t, 0))
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+    };
+
     Piece cur;
     if (!next_piece(cur))
         return;
-    Batch now = batch_of(cur, 0), ahead = batch_of(cur, 32);
+    prefetch_queries(cur);
+    Batch now = batch_of(cur, 0), ahead = now;
+    if (cur.g1 - cur.g0 > 32)
+        ahead = batch_of(cur, 32);
     for (int i = 0; i < min(cur.g1 - cur.g0, kStages); ++i)
         issue(now.at, i);
     const int tok = (r & 1) * 4 + (r >> 1); // MMA row r holds token tok, row r + 8 token tok + 8: then P's columns are tokens q, 4 + q, 8 + q, 12 + q
     const int koff = kv_place<RB>(tok, q * (RB == 32 ? 8 : 16)), voff = kv_place<RB>(q, r * (RB / 8));
     const float inf = INFINITY;
-    const int rows = a.n * a.group;
 
     for (;;) {
         const int head = cur.item / a.row_blocks, row0 = (cur.item - head * a.row_blocks) * kRows;
         const int len = ca_tokens(a, cur.b), ctx = len - a.n;
         // ---- queries: this lane's fragments of the MMA's B operand lie together in global memory, 16 bytes at a time
-        uint2 qr[kQRegs ? NT : 1][kSteps];
+        uint2 qr[NT][kSteps];
         float m[NT][2], l[NT][2], bias[NT][2], O[NT][kTiles][4], rf[NT][2], rs[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -284,11 +313,8 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
             uint4 v[D / 32];
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
-                v[x] = make_uint4(0, 0, 0, 0);
-                // 8 bits: features 16 q .. of each 64; 4 bits: a quarter of the row
-                const int byte = BITS == 8 ? (x >> 1) * 128 + q * 32 + (x & 1) * 16 : q * (D / 2) + x * 16;
-                if (at < rows)
-                    v[x] = *reinterpret_cast<const uint4 *>(a.q + ((long long)cur.b * a.n + i) * a.q_stride + (long long)(head * a.group + at - i * a.group) * a.q_head_stride + byte);
+                const uint8_t *src = query(cur, t, x);
+                v[x] = src ? *reinterpret_cast<const uint4 *>(src) : make_uint4(0, 0, 0, 0);
             }
             float back = 1.f, sum = 0.f;
             if (BF16) {
@@ -324,13 +350,8 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
                 // 8 bits: 4 features a step; 4 bits: a word of 8 codes is two steps, its pairs (1, 5), (0, 4) and (2, 6), (3, 7) apart
                 const uint2 f0 = BITS == 8 ? make_uint2(w[0], w[1]) : make_uint2(__byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632));
                 const uint2 f1 = BITS == 8 ? make_uint2(w[2], w[3]) : make_uint2(__byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632));
-                if (kQRegs) {
-                    qr[kQRegs ? t : 0][2 * x] = f0;
-                    qr[kQRegs ? t : 0][2 * x + 1] = f1;
-                } else {
-                    qfrag[(t * kSteps + 2 * x) * 32 + lane] = f0;
-                    qfrag[(t * kSteps + 2 * x + 1) * 32 + lane] = f1;
-                }
+                qr[t][2 * x] = f0;
+                qr[t][2 * x + 1] = f1;
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -401,8 +422,7 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
                     }
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
-                        const uint2 qq = kQRegs ? qr[kQRegs ? t : 0][k] : qfrag[(t * kSteps + k) * 32 + lane];
-                        mma_f16(s[t], f0, f1, f2, f3, qq.x, qq.y);
+                        mma_f16(s[t], f0, f1, f2, f3, qr[t][k].x, qr[t][k].y);
                     }
                 }
                 const float ks0 = kp[0].x * kKeyScale, ks1 = kp[1].x * kKeyScale;
@@ -545,8 +565,10 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
         Piece next;
         const bool more = next_piece(next);
         if (more) {
+            prefetch_queries(next);
             now = batch_of(next, 0);
-            ahead = batch_of(next, 32);
+            if (next.g1 - next.g0 > 32)
+                ahead = batch_of(next, 32);
             for (int i = 0; i < min(next.g1 - next.g0, kStages); ++i)
                 issue(now.at, i);
         }
@@ -617,8 +639,8 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
     const long long start = prefix * items + (long long)item * ca_units(G);
     int c0 = 0, c1 = 0;
     if (G) {
-        c0 = (int)((start + kCaExtra) / quota);
-        c1 = (int)((start + kCaExtra + G - 1) / quota);
+        c0 = (int)ca_div(start + kCaExtra, quota);
+        c1 = (int)ca_div(start + kCaExtra + G - 1, quota);
         if (c0 == c1)
             return;
     }
@@ -629,8 +651,13 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
     if (row < rows && G) {
         auto slot_of = [&](int c) { return 2 * (size_t)c + (c == c0 && c0 * quota < start ? 1 : 0); };
         float top = -INFINITY;
-        for (int c = c0 + sub; c <= c1; c += kLanes)
-            top = fmaxf(top, ml[slot_of(c) * a.slot_rows + row].x);
+        for (int c = c0 + sub; c <= c1; c += 4 * kLanes) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                x[u] = c + u * kLanes <= c1 ? ml[slot_of(c + u * kLanes) * a.slot_rows + row].x : -INFINITY;
+            top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        }
         const unsigned lanes = kLanes == 16 ? 0xffffu << (threadIdx.x & 16) : 0xffu << (threadIdx.x & 24);
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1)
