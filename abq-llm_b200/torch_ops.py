@@ -8,8 +8,10 @@ and returns without ever calling the launch function.  Here:
 * ``torch.ops.abq_b200.gemm_planes``    -- any WxAy: activation planes x weight planes -> int32 [M][N]
 * ``torch.ops.abq_b200.linear_half``    -- fp16 activations (quantised inside the GEMM call with a static scale) x weight
                                            planes -> fp16 [M][N] through the fused per-channel / per-group dequantisation
+* ``torch.ops.abq_b200.kv_cache_write``, ``kv_cache_read``, ``cache_attention``, ``prompt_attention`` -- the quantised key/value cache and
+                                           attention over it and over whole prompts (include/abq_b200.h has their rules)
 
-Both operators are registered with ``torch.library`` (device "cuda" only: there is no CPU kernel, a CPU tensor is an
+The operators are registered with ``torch.library`` (device "cuda" only: there is no CPU kernel, a CPU tensor is an
 error) together with shape functions, so they can appear in traced graphs.  Scratch memory comes from torch's caching
 allocator, on the current stream.
 """
@@ -78,6 +80,75 @@ def linear_half(x: torch.Tensor, w_planes: torch.Tensor, w_scale: torch.Tensor, 
 @linear_half.register_fake
 def _(x, w_planes, w_scale, w_zero, x_quant_scale, x_bits, w_bits, group_size):
     return x.new_empty((x.shape[0], w_planes.shape[1]), dtype=torch.float16)
+
+
+# ---- attention.  ``cache`` is uint8 [pages][kv_heads][page_size / 16][granule bytes]; ``bits`` 8 or 4; the 16-bit type is that of the other tensors.
+
+def _kv_cache(cache: torch.Tensor, head_dim: int, bits: int, dtype):
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.shape[3] != B.kv_cache_bytes(1, 16, 1, head_dim, bits):
+        raise RuntimeError(f"a cache of {bits} bits and heads of {head_dim} is contiguous uint8 [pages][kv_heads][page_size / 16]"
+                           f"[{B.kv_cache_bytes(1, 16, 1, head_dim, bits)}], not {cache.dtype} {tuple(cache.shape)}")
+    return B.make_kv_cache(cache, page_size=16 * cache.shape[2], kv_heads=cache.shape[1], head_dim=head_dim, bits=bits, dtype=dtype)
+
+
+@torch.library.custom_op(f"{_LIB}::kv_cache_write", mutates_args=("cache",), device_types="cuda")
+def kv_cache_write(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, bits: int) -> None:
+    """Quantise k, v [tokens][kv_heads][head_dim] (fp16 or bf16) and write them to ``slots`` (int64: page * page_size + place, negative = left out)."""
+    _check_cuda(cache, k, v, slots)
+    with torch.cuda.device(k.device):
+        B.kv_cache_write(B.make_kv_write_params(_kv_cache(cache, k.shape[2], bits, k.dtype), k, v, slots))
+
+
+@kv_cache_write.register_fake
+def _(cache, k, v, slots, bits):
+    return None
+
+
+@torch.library.custom_op(f"{_LIB}::kv_cache_read", mutates_args=("k", "v"), device_types="cuda")
+def kv_cache_read(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor, bits: int) -> None:
+    """Whole sequences, packed, into k and v [rows][kv_heads][head_dim]; rows behind the last sequence are left as they were."""
+    _check_cuda(cache, k, v, block_table, cu_seqlens)
+    with torch.cuda.device(k.device):
+        B.kv_cache_read(B.make_kv_read_params(_kv_cache(cache, k.shape[2], bits, k.dtype), k, v, block_table, cu_seqlens))
+
+
+@kv_cache_read.register_fake
+def _(cache, k, v, block_table, cu_seqlens, bits):
+    return None
+
+
+@torch.library.custom_op(f"{_LIB}::cache_attention", mutates_args=(), device_types="cuda")
+def cache_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, tree: torch.Tensor | None, scale: float, bits: int) -> torch.Tensor:
+    """q [batch * n][q_heads][head_dim], the last n tokens of every sequence, over their cached keys and values -> the same shape."""
+    _check_cuda(q, cache, block_table, seq_lens, tree)
+    with torch.cuda.device(q.device):
+        c = _kv_cache(cache, q.shape[2], bits, q.dtype)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        batch = block_table.shape[0]
+        need = B.cache_attention_workspace_bytes(c, batch, q.shape[0] // max(1, batch), q.shape[1])
+        work = torch.empty(max(16, need), dtype=torch.uint8, device=q.device)
+        B.cache_attention(B.make_cache_attention_params(c, q, out, block_table, seq_lens, scale=scale, workspace=work, tree=tree))
+    return out
+
+
+@cache_attention.register_fake
+def _(q, cache, block_table, seq_lens, tree, scale, bits):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::prompt_attention", mutates_args=(), device_types="cuda")
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor, scale: float) -> torch.Tensor:
+    """Causal attention of packed prompts -> [total_q][q_heads][head_dim]; rows behind the last sequence are not written."""
+    _check_cuda(q, k, v, cu_q, cu_k)
+    with torch.cuda.device(q.device):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        B.prompt_attention(B.make_prompt_attention_params(q, k, v, out, cu_q, cu_k, scale=scale))
+    return out
+
+
+@prompt_attention.register_fake
+def _(q, k, v, cu_q, cu_k, scale):
+    return q.new_empty(q.shape)
 
 
 def mul_w2a8(A: torch.Tensor, Bm: torch.Tensor, C: torch.Tensor, prob_m: int, prob_n: int, prob_k: int, sms: int = -1, max_par: int = 8) -> None:

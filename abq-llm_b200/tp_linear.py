@@ -70,11 +70,13 @@ class TensorParallelBlockLinears:
 
     ``backend.make_linear(codes, scale, zero, w_bits, group, reduce_output=...)`` returns an object with
     ``__call__(x_half) -> fp16``; ``backend.all_reduce(t)`` returns the sum over ranks (in ``t`` or in a tensor of its own); ``backend.glue`` supplies the elementwise stand-ins between the
-    GEMMs (attention itself is outside this path: the first third of the QKV output stands in for its result).
+    GEMMs.  ``attention(qkv, out)``, if given (attention.BlockAttention: this rank's heads over a quantised cache), runs between the QKV and
+    the output projection; without it the first third of the QKV output stands in for its result.
     """
 
-    def __init__(self, backend, hidden: int, ffn: int, rank: int, world: int, weights: Sequence, w_bits: int, group: int = 0):
+    def __init__(self, backend, hidden: int, ffn: int, rank: int, world: int, weights: Sequence, w_bits: int, group: int = 0, attention=None):
         self.backend, self.hidden, self.ffn, self.rank, self.world = backend, hidden, ffn, rank, world
+        self.attention = attention
         self.specs = llama_block_specs(hidden, ffn)
         self.layers = {}
         for spec, (codes, scale, zero) in zip(self.specs, weights):
@@ -91,13 +93,18 @@ class TensorParallelBlockLinears:
         # where a layer exposes the buffer its plan reads, the producing elementwise step writes straight into it
         return self.layers[name].input(M) if hasattr(self.layers[name], "input") else None
 
+    def _attention(self, qkv, M):
+        if self.attention is not None:
+            return self.attention(qkv, self._buf("o", M))
+        return self.backend.glue_attention(qkv, self.layers["qkv"].out_features // 3, self._buf("o", M))
+
     # The block in the three pieces that lie between its two all-reduces (a caller that replays CUDA graphs captures
     # the pieces and launches the collectives between them):
     def attention_part(self, x):
         """x -> this rank's partial of the attention output projection (to be all-reduced)."""
         be, M = self.backend, x.shape[0]
         qkv = self.layers["qkv"](x)                                                        # [M][3 * hidden / world]
-        attn = be.glue_attention(qkv, self.layers["qkv"].out_features // 3, self._buf("o", M))  # this rank's heads
+        attn = self._attention(qkv, M)                                                     # this rank's heads
         return self.layers["o"](attn)                                                      # partial [M][hidden]
 
     def ffn_part(self, x, o):
@@ -128,7 +135,7 @@ class TensorParallelBlockLinears:
         output is h + down(act).  Same arithmetic as forward(): the fp16 sum rounded, then an fp16 add."""
         be, M = self.backend, x.shape[0]
         qkv = self.layers["qkv"](x)
-        attn = be.glue_attention(qkv, self.layers["qkv"].out_features // 3, self._buf("o", M))
+        attn = self._attention(qkv, M)
         h = be.linear_sum_plus(self.layers["o"], attn, x, self._buf("gate_up", M), "h")
         gu = self.layers["gate_up"](h)
         act = be.glue_swiglu(gu, self.layers["gate_up"].out_features // 2, self._buf("down", M))
