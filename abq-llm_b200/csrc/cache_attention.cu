@@ -63,6 +63,7 @@ extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, a
     const int rows = a.n * a.group, tiles = row_tiles(rows);
     a.row_blocks = (rows + 8 * tiles - 1) / (8 * tiles);
     a.slot_rows = std::min(rows, 8 * tiles);
+    a.unit_log2 = 4, a.extra = kCaExtra, a.min_quota = kCaMinQuota;
     // the longest sequences that the tables can hold bound the work; real lengths are read on the device
     const long long most = (long long)a.batch * a.kv_heads * a.row_blocks * ((long long)a.table_stride * a.page_granules + kCaExtra);
     a.runs = (int)std::min<long long>((most + kCaMinQuota - 1) / kCaMinQuota, most_runs(tiles));

@@ -31,7 +31,7 @@ constexpr int kCaWarps = 4;
 constexpr int kCaThreads = 32 * kCaWarps;
 constexpr int kCaSms = 148;
 constexpr int kCaMinQuota = 4; // granules a warp takes at least
-constexpr int kCaExtra = 2;
+constexpr int kCaExtra = 2;    // what an item costs beside its granules, in granules
 
 __host__ __device__ constexpr int ca_ctas_per_sm(int tiles) { return tiles == 1 ? 3 : 2; } // 168 or 255 registers a thread
 
@@ -45,6 +45,7 @@ struct CacheAttnArgs {
     float *part; // [2 * runs][slot_rows][D] sums, then [2 * runs][slot_rows] pairs (maximum, sum of p)
     int *status;
     int num_pages, page_granules, kv_heads, batch, n, group, row_blocks, slot_rows, table_stride, runs;
+    int unit_log2, extra, min_quota; // the line's unit: 16 tokens (a warp's granule) or 128 (a CTA's tile)
     float scale_log2;
     unsigned long long page_magic;
 };
@@ -55,15 +56,18 @@ __device__ __forceinline__ int ca_tokens(const CacheAttnArgs &a, int b)
     const int len = a.seq_lens[b];
     return len < 0 ? 0 : (int)min((long long)min(len, 0x7fffff00), cap);
 }
-__device__ __forceinline__ int ca_granules(const CacheAttnArgs &a, int b) { return (int)(((long long)ca_tokens(a, b) + 15) >> 4); }
-__device__ __forceinline__ int ca_units(int granules) { return granules ? granules + kCaExtra : 0; } // an item's length on the line
+__device__ __forceinline__ int ca_granules(const CacheAttnArgs &a, int b) // (or tiles: units)
+{
+    return (int)(((long long)ca_tokens(a, b) + (1 << a.unit_log2) - 1) >> a.unit_log2);
+}
+__device__ __forceinline__ int ca_units(const CacheAttnArgs &a, int granules) { return granules ? granules + a.extra : 0; } // an item's length on the line
 
 // Units of all sequences, and of those before sequence `before`, one item each; by a warp.
 __device__ __forceinline__ void ca_sums(const CacheAttnArgs &a, int before, long long &all, long long &prefix)
 {
     long long s = 0, p = 0;
     for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
-        const int u = ca_units(ca_granules(a, b));
+        const int u = ca_units(a, ca_granules(a, b));
         s += u;
         p += b < before ? u : 0;
     }
@@ -80,9 +84,85 @@ __device__ __forceinline__ long long ca_div(long long x, long long y)
 {
     return ((unsigned long long)(x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y;
 }
-__device__ __forceinline__ long long ca_quota(const CacheAttnArgs &a, long long total) { return max(ca_div(total + a.runs - 1, a.runs), (long long)kCaMinQuota); }
+__device__ __forceinline__ long long ca_quota(const CacheAttnArgs &a, long long total) { return max(ca_div(total + a.runs - 1, a.runs), (long long)a.min_quota); }
 // Entry of a block table that holds granule g (page_magic = ceil(2^34 / page_granules): exact for granule numbers below 2^28)
 __device__ __forceinline__ int ca_entry(const CacheAttnArgs &a, int g) { return (int)(((unsigned long long)(uint32_t)g * a.page_magic) >> 34); }
+
+// A part of an item that one run holds, and the walk over a run's parts (by a warp, all lanes alike).
+struct CaPiece {
+    int b, item, G, g0, g1; // units g0 .. g1 - 1 of G
+    bool first;             // the run starts in this item
+};
+struct CaRun {
+    int b, G, item, pos;
+    long long left;
+    bool first;
+
+    __device__ __forceinline__ bool begin(const CacheAttnArgs &a, int run, int lane)
+    {
+        const int items = a.kv_heads * a.row_blocks;
+        long long units = 0, quota = 0, rem = 0, unused;
+        first = true;
+        if (a.batch > 32) {
+            ca_sums(a, 0, units, unused);
+            quota = ca_quota(a, units * items);
+        }
+        for (int b0 = 0;; b0 += 32) { // 32 sequences at a time
+            const int own = b0 + lane < a.batch ? ca_granules(a, b0 + lane) : 0;
+            uint32_t upto = ca_units(a, own);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+                upto += lane >= o ? x : 0;
+            }
+            if (b0 == 0) {
+                if (a.batch <= 32) {
+                    units = __shfl_sync(0xffffffffu, upto, 31);
+                    quota = ca_quota(a, units * items);
+                }
+                rem = run * quota; // from the start of sequence b0
+                left = min(units * items, rem + quota) - rem;
+                if (left <= 0)
+                    return false;
+            }
+            const uint32_t behind = __ballot_sync(0xffffffffu, rem < (long long)upto * items);
+            if (behind) {
+                const int at = __ffs(behind) - 1;
+                b = b0 + at;
+                G = __shfl_sync(0xffffffffu, own, at);
+                rem -= (long long)(__shfl_sync(0xffffffffu, upto, at) - ca_units(a, G)) * items;
+                break;
+            }
+            rem -= (long long)__shfl_sync(0xffffffffu, upto, 31) * items;
+        }
+        item = (int)ca_div(rem, ca_units(a, G));
+        pos = (int)(rem - (long long)item * ca_units(a, G));
+        return true;
+    }
+    __device__ __forceinline__ bool next(const CacheAttnArgs &a, CaPiece &p) // the next part that has units
+    {
+        while (left > 0) {
+            if (pos == ca_units(a, G)) {
+                pos = 0;
+                first = false;
+                if (++item == a.kv_heads * a.row_blocks) {
+                    item = 0;
+                    do {
+                        G = ca_granules(a, ++b);
+                    } while (G == 0);
+                }
+            }
+            const int span = (int)min((long long)(ca_units(a, G) - pos), left);
+            p.b = b, p.item = item, p.G = G, p.first = first;
+            p.g0 = max(0, pos - a.extra), p.g1 = max(0, pos + span - a.extra);
+            pos += span;
+            left -= span;
+            if (p.g1 > p.g0)
+                return true;
+        }
+        return false;
+    }
+};
 
 __device__ __forceinline__ float ex2(float x)
 {
@@ -169,53 +249,13 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
     pdl_launch_dependents();
     pdl_wait_prior_grid();
 
-    // ---- this warp's run of the line
-    const int items = a.kv_heads * a.row_blocks, run = blockIdx.x * kCaWarps + warp;
-    int b = 0, G = 0, item, pos;
-    long long left;
-    {
-        long long units = 0, quota = 0, rem = 0, unused;
-        if (a.batch > 32) {
-            ca_sums(a, 0, units, unused);
-            quota = ca_quota(a, units * items);
-        }
-        for (int b0 = 0;; b0 += 32) { // 32 sequences at a time
-            const int own = b0 + lane < a.batch ? ca_granules(a, b0 + lane) : 0;
-            uint32_t upto = ca_units(own);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
-                upto += lane >= o ? x : 0;
-            }
-            if (b0 == 0) {
-                if (a.batch <= 32) {
-                    units = __shfl_sync(0xffffffffu, upto, 31);
-                    quota = ca_quota(a, units * items);
-                }
-                rem = run * quota; // from the start of sequence b0
-                left = min(units * items, rem + quota) - rem;
-                if (left <= 0)
-                    return; // (before any copy)
-            }
-            const uint32_t behind = __ballot_sync(0xffffffffu, rem < (long long)upto * items);
-            if (behind) {
-                const int at = __ffs(behind) - 1;
-                b = b0 + at;
-                G = __shfl_sync(0xffffffffu, own, at);
-                rem -= (long long)(__shfl_sync(0xffffffffu, upto, at) - ca_units(G)) * items;
-                break;
-            }
-            rem -= (long long)__shfl_sync(0xffffffffu, upto, 31) * items;
-        }
-        item = (int)ca_div(rem, ca_units(G));
-        pos = (int)(rem - (long long)item * ca_units(G));
-    }
+    const int run = blockIdx.x * kCaWarps + warp;
+    CaRun line;
+    if (!line.begin(a, run, lane))
+        return; // (before any copy)
 
     // ---- ring of granules: lane i % 32 owns the address of granule i of the piece
-    struct Piece {
-        int b, item, G, g0, g1;
-        bool first;
-    };
+    using Piece = CaPiece;
     struct Batch {
         uint32_t at;   // index of the granule in the cache, or ~0
         uint32_t good; // ballot: which of the 32 lie in the cache
@@ -249,30 +289,6 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
         }
         put_stage = put_stage + 1 == kStages ? 0 : put_stage + 1;
     };
-    bool first = true;
-    auto next_piece = [&](Piece &p) { // the next part of the run that has granules
-        while (left > 0) {
-            if (pos == ca_units(G)) {
-                pos = 0;
-                first = false;
-                if (++item == items) {
-                    item = 0;
-                    do {
-                        G = ca_granules(a, ++b);
-                    } while (G == 0);
-                }
-            }
-            const int span = (int)min((long long)(ca_units(G) - pos), left);
-            p.b = b, p.item = item, p.G = G, p.first = first;
-            p.g0 = max(0, pos - kCaExtra), p.g1 = max(0, pos + span - kCaExtra);
-            pos += span;
-            left -= span;
-            if (p.g1 > p.g0)
-                return true;
-        }
-        return false;
-    };
-
     const int rows = a.n * a.group;
     // the 16 bytes x of this lane's queries in tile t of an item
     auto query = [&](const Piece &p, int t, int x) -> const uint8_t * {
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
     };
 
     Piece cur;
-    if (!next_piece(cur))
+    if (!line.next(a, cur))
         return;
     prefetch_queries(cur);
     Batch now = batch_of(cur, 0), ahead = now;
@@ -563,7 +579,7 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
 
         // ---- the next piece's first copies go out before this one's result is written
         Piece next;
-        const bool more = next_piece(next);
+        const bool more = line.next(a, next);
         if (more) {
             prefetch_queries(next);
             now = batch_of(next, 0);
@@ -636,11 +652,11 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
     ca_sums(a, b, units, prefix);
     const long long quota = ca_quota(a, units * items);
     const int G = ca_granules(a, b);
-    const long long start = prefix * items + (long long)item * ca_units(G);
+    const long long start = prefix * items + (long long)item * ca_units(a, G);
     int c0 = 0, c1 = 0;
     if (G) {
-        c0 = (int)ca_div(start + kCaExtra, quota);
-        c1 = (int)ca_div(start + kCaExtra + G - 1, quota);
+        c0 = (int)ca_div(start + a.extra, quota);
+        c1 = (int)ca_div(start + a.extra + G - 1, quota);
         if (c0 == c1)
             return;
     }
