@@ -10,11 +10,26 @@ cudaError_t launch_cache_attention(const CacheAttnArgs &args, int head_dim, int 
 extern template cudaError_t launch_cache_attention<1>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
 extern template cudaError_t launch_cache_attention<2>(const CacheAttnArgs &, int, int, bool, cudaStream_t);
 
-// Tiles of 8 query rows that a block holds.  One conversion of the codes serves them all, but with more rows fewer warps fit: blocks of 16 measured faster than
-// of 32 for 26 rows over 40 heads of 128, 8 bits (36.8 and 43.5 us; blocks of 8: 41.8), and nearly as fast for 256 rows of 64, 4 bits (57.4 and 53.7).
+// Tiles of 8 query rows that a block of the mma.sync kernel holds.  One conversion of the codes serves them all, but with more rows fewer warps fit: blocks of 16
+// measured faster than of 32 for 26 rows over 40 heads of 128, 8 bits (36.8 and 43.5 us; blocks of 8: 41.8).
 static int row_tiles(int rows) { return rows <= 8 ? 1 : 2; }
 
-static int most_runs(int tiles) { return kCaSms * ca_ctas_per_sm(tiles) * kCaWarps; }
+cudaError_t launch_cache_attention_tile(const CacheAttnArgs &args, int head_dim, int bits, bool bf16, cudaStream_t stream);
+
+// What a call of so many query rows a head runs on.
+struct CaPlan {
+    bool tile;              // the kernel of 128 rows (cache_attention_tile.cu)
+    int block, most_runs;   // rows of a block; runs the line is cut into at most
+    int unit_log2, extra, min_quota;
+};
+static CaPlan ca_plan(int rows)
+{
+    const int blocks = (rows + 127) / 128;
+    if (rows >= 96 && 4 * rows >= 3 * 128 * blocks) // (measured: see there)
+        return { true, 128, kCaSms, 7, 1, 2 };
+    const int tiles = row_tiles(rows);
+    return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(tiles) * kCaWarps, 4, kCaExtra, kCaMinQuota };
+}
 
 static bool attention_shape_valid(const abq_kv_cache &c, int batch, int n, int q_heads)
 {
@@ -30,8 +45,9 @@ extern "C" size_t abq_cache_attention_workspace_bytes(const abq_kv_cache *cache,
     using namespace abq;
     if (!cache || !attention_shape_valid(*cache, batch, rows_per_seq, q_heads))
         return 0;
-    const int rows = rows_per_seq * (q_heads / cache->kv_heads), tiles = row_tiles(rows);
-    return (size_t)2 * most_runs(tiles) * std::min(rows, 8 * tiles) * (cache->head_dim + 2) * sizeof(float);
+    const int rows = rows_per_seq * (q_heads / cache->kv_heads);
+    const CaPlan plan = ca_plan(rows);
+    return (size_t)2 * plan.most_runs * std::min(rows, plan.block) * (cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, abq_stream_t stream)
@@ -60,17 +76,21 @@ extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, a
     a.group = p->q_heads / p->cache.kv_heads, a.table_stride = p->table_stride;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.page_magic = ((1ull << 34) + a.page_granules - 1) / a.page_granules;
-    const int rows = a.n * a.group, tiles = row_tiles(rows);
-    a.row_blocks = (rows + 8 * tiles - 1) / (8 * tiles);
-    a.slot_rows = std::min(rows, 8 * tiles);
-    a.unit_log2 = 4, a.extra = kCaExtra, a.min_quota = kCaMinQuota;
+    const int rows = a.n * a.group;
+    const CaPlan plan = ca_plan(rows);
+    a.row_blocks = (rows + plan.block - 1) / plan.block;
+    a.slot_rows = std::min(rows, plan.block);
+    a.unit_log2 = plan.unit_log2, a.extra = plan.extra, a.min_quota = plan.min_quota;
     // the longest sequences that the tables can hold bound the work; real lengths are read on the device
-    const long long most = (long long)a.batch * a.kv_heads * a.row_blocks * ((long long)a.table_stride * a.page_granules + kCaExtra);
-    a.runs = (int)std::min<long long>((most + kCaMinQuota - 1) / kCaMinQuota, most_runs(tiles));
+    const long long units = (((long long)a.table_stride * p->cache.page_size + (1 << a.unit_log2) - 1) >> a.unit_log2) + a.extra;
+    const long long most = (long long)a.batch * a.kv_heads * a.row_blocks * units;
+    a.runs = (int)std::min<long long>((most + a.min_quota - 1) / a.min_quota, plan.most_runs);
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int D = p->cache.head_dim, bits = p->cache.bits;
     const bool bf16 = p->cache.half_type == ABQ_HALF_BF16;
-    const cudaError_t e = tiles == 1 ? launch_cache_attention<1>(a, D, bits, bf16, s) : launch_cache_attention<2>(a, D, bits, bf16, s);
+    const cudaError_t e = plan.tile        ? launch_cache_attention_tile(a, D, bits, bf16, s)
+                          : plan.block == 8 ? launch_cache_attention<1>(a, D, bits, bf16, s)
+                                            : launch_cache_attention<2>(a, D, bits, bf16, s);
     if (e != cudaSuccess) {
         set_last_cuda_error(e);
         return ABQ_ERR_CUDA;

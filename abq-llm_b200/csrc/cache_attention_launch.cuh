@@ -20,6 +20,18 @@ cudaError_t launch_chained(Kernel kern, dim3 grid, size_t smem, cudaStream_t str
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+template <int D, bool BF16>
+cudaError_t launch_cache_attention_combine(const CacheAttnArgs &args, int block_rows, cudaStream_t stream)
+{
+    constexpr int kGroups = kCaThreads / (D / 8);
+    // rows of a block at a time: few (the other groups of threads take pieces in turn) where the items alone do not fill the GPU
+    const long long items = (long long)args.batch * args.kv_heads * args.row_blocks;
+    int rows = 1;
+    while (rows < args.slot_rows && rows < kGroups && items * args.slot_rows / rows > 4 * kCaSms)
+        rows *= 2;
+    return launch_chained(cache_attention_combine_kernel<D, BF16>, dim3((unsigned)items, (args.slot_rows + rows - 1) / rows), 0, stream, args, block_rows, rows);
+}
+
 template <int D, int BITS, int NT, bool BF16>
 cudaError_t launch_cache_attention_as(const CacheAttnArgs &args, cudaStream_t stream)
 {
@@ -29,15 +41,7 @@ cudaError_t launch_cache_attention_as(const CacheAttnArgs &args, cudaStream_t st
     cudaError_t e = opted.ensure(kern, smem);
     if (e == cudaSuccess)
         e = launch_chained(kern, dim3((args.runs + kCaWarps - 1) / kCaWarps), smem, stream, args);
-    if (e != cudaSuccess)
-        return e;
-    constexpr int kGroups = kCaThreads / (D / 8);
-    // rows of a block at a time: few (the other groups of threads take pieces in turn) where the items alone do not fill the GPU
-    const long long items = (long long)args.batch * args.kv_heads * args.row_blocks;
-    int rows = 1;
-    while (rows < args.slot_rows && rows < kGroups && items * args.slot_rows / rows > 4 * kCaSms)
-        rows *= 2;
-    return launch_chained(cache_attention_combine_kernel<D, BF16>, dim3((unsigned)items, (args.slot_rows + rows - 1) / rows), 0, stream, args, 8 * NT, rows);
+    return e != cudaSuccess ? e : launch_cache_attention_combine<D, BF16>(args, 8 * NT, stream);
 }
 
 template <int NT>

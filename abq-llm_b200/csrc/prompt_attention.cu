@@ -26,6 +26,7 @@
 #include <type_traits>
 
 #include "abq_kernels.h"
+#include "attention_tmem.cuh"
 #include "kv_cache.cuh"
 #include "umma.cuh"
 
@@ -155,38 +156,6 @@ __device__ __forceinline__ PaItem pa_item(const PaArgs &a, int idx, int lane)
 __device__ __forceinline__ int pa_k_place(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int pa_v_place(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
 
-__device__ __forceinline__ float pa_ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float pa_max3(float a, float b, float c)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); // (keeps NaN)
-    return r;
-}
-__device__ __forceinline__ uint64_t pa_pack(float lo, float hi)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void pa_unpack(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b)
-{
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // 2^x of two numbers of at most 2^14; below 2^-125 it stays there.  NaN is lost: the caller looks for it.
 template <bool BF16>
 __device__ __forceinline__ void pa_ex2_poly(uint64_t x2, float &lo, float &hi)
@@ -214,44 +183,6 @@ __device__ __forceinline__ void pa_ex2_poly(uint64_t x2, float &lo, float &hi)
     lo = __int_as_float(__float_as_int(lo) + (__float_as_int(n0) << 23));
     hi = __int_as_float(__float_as_int(hi) + (__float_as_int(n1) << 23));
 }
-
-#define PA_REGS32(v)                                                                                                                                       \
-    "+f"((v)[0]), "+f"((v)[1]), "+f"((v)[2]), "+f"((v)[3]), "+f"((v)[4]), "+f"((v)[5]), "+f"((v)[6]), "+f"((v)[7]), "+f"((v)[8]), "+f"((v)[9]),           \
-        "+f"((v)[10]), "+f"((v)[11]), "+f"((v)[12]), "+f"((v)[13]), "+f"((v)[14]), "+f"((v)[15]), "+f"((v)[16]), "+f"((v)[17]), "+f"((v)[18]),             \
-        "+f"((v)[19]), "+f"((v)[20]), "+f"((v)[21]), "+f"((v)[22]), "+f"((v)[23]), "+f"((v)[24]), "+f"((v)[25]), "+f"((v)[26]), "+f"((v)[27]),             \
-        "+f"((v)[28]), "+f"((v)[29]), "+f"((v)[30]), "+f"((v)[31])
-
-// 32 accumulator columns of this thread's TMEM lane; the values may be used after pa_ld_wait() on them
-__device__ __forceinline__ void pa_ld32(uint32_t taddr, float *v)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
-                   "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
-                   "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-                 : "r"(taddr));
-}
-__device__ __forceinline__ void pa_ld_wait(float *v) { asm volatile("tcgen05.wait::ld.sync.aligned;" : PA_REGS32(v)::"memory"); }
-__device__ __forceinline__ void pa_ld16(uint32_t taddr, float *v)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
-                   "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void pa_ld_tie(float *v) { asm volatile("" : PA_REGS32(v)); } // (waited for with others)
-__device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t *v)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(v[0]),
-                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
-                 "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
-__device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 16-byte pieces w[0..3] of four neighbouring lanes: lane b of them ends with piece b of lane k in w[k]
 __device__ __forceinline__ void transpose4(uint32_t (&w)[4][4], int lane)

@@ -80,7 +80,7 @@ def test_cache_attention_refuses(abq):
     _refused(fn, abq.CacheAttentionParams, good, [dict(workspace=None), dict(workspace=4104), dict(workspace_bytes=need - 1)], WORKSPACE)
     for rows, heads in ((0, 4), (65, 4), (1, 3), (1, 0)):
         assert abq.cache_attention_workspace_bytes(c, 2, rows, heads) == 0
-    assert abq.cache_attention_workspace_bytes(c, 2, 16, 4) >= abq.cache_attention_workspace_bytes(c, 2, 8, 4) > need
+    assert abq.cache_attention_workspace_bytes(c, 2, 8, 4) > need and abq.cache_attention_workspace_bytes(c, 2, 64, 4) > need
 
 
 def test_prompt_attention_refuses(abq):

@@ -77,13 +77,19 @@ class Setup:
     (2, 1, 64, [64, 200, 63, 1], 16, True),
     (16, 2, 9, [500, 12], 16, True),
     (12, 12, 1, [257] * 9 + [0, 3], 16, False),
+    # blocks of 128 rows on the tensor cores: 96, 128, 192 (two blocks) and 256 rows
+    (8, 2, 24, [24, 23, 150, 0, 300], 32, True),
+    (8, 1, 16, [1, 17, 128, 129, 1500], 16, False),
+    (12, 1, 16, [333, 16], 48, True),
+    (8, 2, 64, [64, 700, 1, 128], 128, True),
+    (16, 2, 16, [200] * 35 + [0, 5], 16, False),
 ])
 def test_against_64_bits(abq, cuda, dim, bits, half, heads, kv_heads, n, lens, page, tree):
     s = Setup(abq, dim=dim, bits=bits, half=HALF[half], heads=heads, kv_heads=kv_heads, n=n, lens=lens, page=page, tree=tree, seed=len(lens) + dim + n).fill()
     s.check(s.call())
 
 
-@pytest.mark.parametrize("bits,heads,kv_heads,n,lens", [(8, 8, 8, 1, [5000]), (4, 32, 4, 1, [3001, 7, 2048, 4000]), (8, 4, 1, 20, [6100, 900])])
+@pytest.mark.parametrize("bits,heads,kv_heads,n,lens", [(8, 8, 8, 1, [5000]), (4, 32, 4, 1, [3001, 7, 2048, 4000]), (8, 4, 1, 20, [6100, 900]), (8, 8, 1, 16, [9000, 300])])
 def test_sequences_that_many_blocks_share(abq, cuda, bits, heads, kv_heads, n, lens):
     s = Setup(abq, dim=128, bits=bits, half=torch.float16, heads=heads, kv_heads=kv_heads, n=n, lens=lens, page=16, tree=n > 1, seed=bits).fill()
     first = s.call().clone()
@@ -92,9 +98,10 @@ def test_sequences_that_many_blocks_share(abq, cuda, bits, heads, kv_heads, n, l
     assert torch.equal(first, s.out), "the same bits again: pieces are added in order"
 
 
-def test_rows_that_see_nothing_and_masked_nan(abq, cuda):
+@pytest.mark.parametrize("heads", [2, 48])
+def test_rows_that_see_nothing_and_masked_nan(abq, cuda, heads):
     """Tree rows without a bit and nothing before the drafts give 0; drafts whose keys and values are NaN touch only the rows that see them."""
-    s = Setup(abq, dim=64, bits=8, half=torch.float16, heads=2, kv_heads=2, n=4, lens=[4, 30], page=16, tree=True, seed=3)
+    s = Setup(abq, dim=64, bits=8, half=torch.float16, heads=heads, kv_heads=2, n=4, lens=[4, 30], page=16, tree=True, seed=3)
     s.tree[0] = torch.tensor([0, 2, 0, 8])
     s.tree[1] = torch.tensor([1, 2, 5, 9])
     s.k[4 + 27], s.v[4 + 27] = float("nan"), float("inf")  # sequence 1, draft 1: seen by row 1 alone
@@ -106,11 +113,12 @@ def test_rows_that_see_nothing_and_masked_nan(abq, cuda):
     s.check(out, rows=[0, 1, 2, 3, 4, 6, 7])
 
 
-def test_many_small_weights_beside_one_large(abq, cuda):
+@pytest.mark.parametrize("n", [1, 64])
+def test_many_small_weights_beside_one_large(abq, cuda, n):
     """One key draws almost all weight; 20000 others together hold a part that must not be lost when their weights are held in 16 bits."""
     for half in (torch.float16, torch.bfloat16):
         torch.manual_seed(4)
-        s = Setup(abq, dim=64, bits=8, half=half, heads=1, kv_heads=1, n=1, lens=[20001], page=16)
+        s = Setup(abq, dim=64, bits=8, half=half, heads=2 if n > 1 else 1, kv_heads=1, n=n, lens=[20001], page=16)
         s.q[:] = 1.0
         s.k = torch.zeros_like(s.k)
         s.k[:, 0, 0] = torch.rand(20001) * 0.01  # (codes of their own)
@@ -120,34 +128,38 @@ def test_many_small_weights_beside_one_large(abq, cuda):
         s.fill()
         out = s.call()
         s.check(out)
-        want, _ = R.cache_attention(s.data, 16, 8, half, s.table, s.lens, s.q, 1, s.scale)
+        want, _ = R.cache_attention(s.data, 16, 8, half, s.table, s.lens, s.q, n, s.scale)
         # the others' share is 20000 exp(-1.9 * 64 / 8) = 0.0050, their values lie 2 away: 0.00998, many steps of the result's type
         assert float((want - (-1.0)).abs().min()) > 0.009, "the case says nothing if the small ones do not count"
 
 
-def test_value_scales_of_all_sizes(abq, cuda):
+@pytest.mark.parametrize("heads,n", [(4, 1), (4, 32)])
+def test_value_scales_of_all_sizes(abq, cuda, heads, n):
     """Value rows from 2^-14 to 2^14 of the first: the power of two that holds p times the scale in 16 bits follows the largest."""
-    s = Setup(abq, dim=128, bits=8, half=torch.bfloat16, heads=4, kv_heads=1, n=1, lens=[700], page=16, seed=5)
+    s = Setup(abq, dim=128, bits=8, half=torch.bfloat16, heads=heads, kv_heads=1, n=n, lens=[700], page=16, seed=5)
     s.v = (s.v.float() * 2.0 ** torch.randint(-14, 15, (700, 1, 1), generator=torch.Generator().manual_seed(1)).float()).to(torch.bfloat16)
     s.v[:40] = 0.5  # constant rows first: scale 0
     s.fill()
     s.check(s.call())
 
 
-def test_queries_of_all_sizes(abq, cuda):
-    s = Setup(abq, dim=128, bits=8, half=torch.bfloat16, heads=6, kv_heads=1, n=1, lens=[100], page=16, seed=6)
+@pytest.mark.parametrize("n", [1, 16])
+def test_queries_of_all_sizes(abq, cuda, n):
+    s = Setup(abq, dim=128, bits=8, half=torch.bfloat16, heads=6, kv_heads=1, n=n, lens=[100], page=16, seed=6)
     s.q[0] *= torch.tensor([1e-30, 1e-3, 1.0, 50.0, 0.0, 3e-39]).view(6, 1).to(torch.bfloat16)
     s.fill()
     s.check(s.call())
 
 
-def test_in_place(abq, cuda):
-    s = Setup(abq, dim=128, bits=4, half=torch.float16, heads=8, kv_heads=2, n=3, lens=[900, 31], page=16, tree=True, seed=8).fill()
+@pytest.mark.parametrize("heads", [8, 64])
+def test_in_place(abq, cuda, heads):
+    s = Setup(abq, dim=128, bits=4, half=torch.float16, heads=heads, kv_heads=2, n=3, lens=[900, 31], page=16, tree=True, seed=8).fill()
     s.check(s.call(out="q"))
 
 
-def test_pages_outside_the_cache_are_unseen(abq, cuda):
-    s = Setup(abq, dim=64, bits=8, half=torch.float16, heads=2, kv_heads=2, n=1, lens=[64], page=16, seed=9).fill()
+@pytest.mark.parametrize("heads", [2, 256])
+def test_pages_outside_the_cache_are_unseen(abq, cuda, heads):
+    s = Setup(abq, dim=64, bits=8, half=torch.float16, heads=heads, kv_heads=2, n=1, lens=[64], page=16, seed=9).fill()
     whole = s.table.clone()
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     s.call(status=status)
@@ -170,8 +182,9 @@ def test_pages_outside_the_cache_are_unseen(abq, cuda):
     assert torch.equal(long, s.call())
 
 
-def test_a_captured_launch_follows_the_lengths(abq, cuda):
-    s = Setup(abq, dim=128, bits=8, half=torch.float16, heads=8, kv_heads=2, n=1, lens=[400, 90], page=16, seed=10).fill()
+@pytest.mark.parametrize("heads", [8, 192])
+def test_a_captured_launch_follows_the_lengths(abq, cuda, heads):
+    s = Setup(abq, dim=128, bits=8, half=torch.float16, heads=heads, kv_heads=2, n=1, lens=[400, 90], page=16, seed=10).fill()
     s.call()
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
@@ -187,9 +200,10 @@ def test_a_captured_launch_follows_the_lengths(abq, cuda):
         s.check(s.out)
 
 
-def test_two_streams_with_workspaces_of_their_own(abq, cuda):
-    a = Setup(abq, dim=128, bits=8, half=torch.float16, heads=8, kv_heads=8, n=1, lens=[3000], page=16, seed=11).fill()
-    b = Setup(abq, dim=128, bits=8, half=torch.float16, heads=8, kv_heads=8, n=1, lens=[2900], page=16, seed=12).fill()
+@pytest.mark.parametrize("heads,kv_heads,n", [(8, 8, 1), (16, 2, 16)])
+def test_two_streams_with_workspaces_of_their_own(abq, cuda, heads, kv_heads, n):
+    a = Setup(abq, dim=128, bits=8, half=torch.float16, heads=heads, kv_heads=kv_heads, n=n, lens=[3000], page=16, seed=11).fill()
+    b = Setup(abq, dim=128, bits=8, half=torch.float16, heads=heads, kv_heads=kv_heads, n=n, lens=[2900], page=16, seed=12).fill()
     a.call(run=False), b.call(run=False)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
