@@ -376,6 +376,35 @@ def _ints(t, shape, what: str, dtype: str = "int32"):
     return t.data_ptr()
 
 
+def _one_device(**tensors) -> int:
+    """Index of the device that all of them (but None and plain addresses) are on: a kernel must not be handed another GPU's memory."""
+    found = {name: t.device.index for name, t in tensors.items() if t is not None and not isinstance(t, int)}
+    if len(set(found.values())) > 1:
+        raise ValueError("tensors on different devices: " + ", ".join(f"{name} on cuda:{index}" for name, index in found.items()))
+    return next(iter(found.values()))
+
+
+_current_device = None
+
+
+def _launch(entry: str, params, stream) -> None:
+    """The call on the device its tensors are on, whichever is current; ``stream`` None: that device's current stream."""
+    global _current_device
+    if _current_device is None:
+        import torch
+        torch.cuda.init()
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    call = getattr(_lib or lib(), entry)
+    if params._device == _current_device():
+        status = call(ctypes.byref(params), _raw_stream(stream))
+    else:
+        import torch
+        with torch.cuda.device(params._device):
+            status = call(ctypes.byref(params), _raw_stream(stream))
+    if status:
+        _check(status, entry)
+
+
 def kv_cache_bytes(num_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int) -> int:
     """Bytes of one layer's cache (0: no such cache)."""
     return int(lib().abq_kv_cache_bytes(ctypes.byref(KVCache(None, num_pages, page_size, kv_heads, head_dim, bits, HALF_FP16))))
@@ -401,14 +430,13 @@ def make_kv_write_params(cache: KVCache, k, v, slots) -> KVWriteParams:
     if v.shape[0] != p.tokens:
         raise ValueError(f"{p.tokens} rows of k, {v.shape[0]} of v")
     p.slots = _ints(slots, (p.tokens,), "slots", "int64")
+    p._device = _one_device(cache=cache._keep_alive, k=k, v=v, slots=slots)
     p._keep_alive = (cache, k, v, slots)
     return p
 
 
 def kv_cache_write(params: KVWriteParams, stream=None) -> None:
-    status = (_lib or lib()).abq_kv_cache_write(ctypes.byref(params), _raw_stream(stream))
-    if status:
-        _check(status, "abq_kv_cache_write")
+    _launch("abq_kv_cache_write", params, stream)
 
 
 def make_kv_read_params(cache: KVCache, k, v, block_table, cu_seqlens) -> KVReadParams:
@@ -422,14 +450,13 @@ def make_kv_read_params(cache: KVCache, k, v, block_table, cu_seqlens) -> KVRead
     p.batch, p.table_stride = block_table.shape
     p.block_table = _ints(block_table, (p.batch, p.table_stride), "block_table")
     p.cu_seqlens = _ints(cu_seqlens, (p.batch + 1,), "cu_seqlens")
+    p._device = _one_device(cache=cache._keep_alive, k=k, v=v, block_table=block_table, cu_seqlens=cu_seqlens)
     p._keep_alive = (cache, k, v, block_table, cu_seqlens)
     return p
 
 
 def kv_cache_read(params: KVReadParams, stream=None) -> None:
-    status = (_lib or lib()).abq_kv_cache_read(ctypes.byref(params), _raw_stream(stream))
-    if status:
-        _check(status, "abq_kv_cache_read")
+    _launch("abq_kv_cache_read", params, stream)
 
 
 def cache_attention_workspace_bytes(cache: KVCache, batch: int, rows_per_seq: int, q_heads: int) -> int:
@@ -453,14 +480,13 @@ def make_cache_attention_params(cache: KVCache, q, out, block_table, seq_lens, *
     p.scale = scale
     p.workspace, p.workspace_bytes = _ptr(workspace), workspace.numel() * workspace.element_size()
     p.status_word = _ptr(status_word)
+    p._device = _one_device(cache=cache._keep_alive, q=q, out=out, block_table=block_table, seq_lens=seq_lens, tree=tree, workspace=workspace, status_word=status_word)
     p._keep_alive = (cache, q, out, block_table, seq_lens, tree, workspace, status_word)
     return p
 
 
 def cache_attention(params: CacheAttentionParams, stream=None) -> None:
-    status = (_lib or lib()).abq_cache_attention(ctypes.byref(params), _raw_stream(stream))
-    if status:
-        _check(status, "abq_cache_attention")
+    _launch("abq_cache_attention", params, stream)
 
 
 def make_prompt_attention_params(q, k, v, out, cu_q, cu_k, *, scale: float, max_q: int = 0, status_word=None) -> PromptAttentionParams:
@@ -478,11 +504,10 @@ def make_prompt_attention_params(q, k, v, out, cu_q, cu_k, *, scale: float, max_
     p.batch = cu_q.numel() - 1
     p.cu_q, p.cu_k = _ints(cu_q, (p.batch + 1,), "cu_q"), _ints(cu_k, (p.batch + 1,), "cu_k")
     p.scale, p.max_q, p.status_word = scale, max_q, _ptr(status_word)
+    p._device = _one_device(q=q, k=k, v=v, out=out, cu_q=cu_q, cu_k=cu_k, status_word=status_word)
     p._keep_alive = (q, k, v, out, cu_q, cu_k, status_word)
     return p
 
 
 def prompt_attention(params: PromptAttentionParams, stream=None) -> None:
-    status = (_lib or lib()).abq_prompt_attention(ctypes.byref(params), _raw_stream(stream))
-    if status:
-        _check(status, "abq_prompt_attention")
+    _launch("abq_prompt_attention", params, stream)

@@ -111,3 +111,38 @@ def test_python_layer_refuses(abq):
         abq.make_kv_read_params(c, x[..., :64], x, torch.zeros((1, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError, match="same rows"):
         abq.make_cache_attention_params(c, x, x, torch.zeros((2, 1), dtype=torch.int32), torch.zeros(2, dtype=torch.int32), scale=1.0, workspace=x)
+
+
+def test_tensors_of_one_call_are_on_one_device(abq):
+    from types import SimpleNamespace as NS
+    on = lambda i: NS(device=NS(index=i))  # noqa: E731
+    assert abq.binding._one_device(q=on(1), k=on(1), tree=None, status_word=4096) == 1
+    with pytest.raises(ValueError, match="different devices.*q on cuda:0.*table on cuda:1"):
+        abq.binding._one_device(q=on(0), table=on(1))
+
+
+def test_calls_go_to_the_device_of_their_tensors(abq, monkeypatch):
+    """The call is made with the tensors' device current, on that device's stream, and the old one is current behind it."""
+    import torch
+    from types import SimpleNamespace as NS
+    now, seen = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.old, now[0] = now[0], self.index
+
+        def __exit__(self, *e):
+            now[0] = self.old
+
+    monkeypatch.setattr(abq.binding, "_current_device", lambda: now[0])
+    monkeypatch.setattr(abq.binding, "_current_raw", lambda: 100 + now[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(abq.binding, "_lib", NS(abq_kv_cache_write=lambda p, stream: seen.append((now[0], stream)) or 0))
+    for device in (0, 1):
+        p = abq.binding.KVWriteParams()
+        p._device = device
+        abq.kv_cache_write(p)
+    assert seen == [(0, 100), (1, 101)] and now == [0]
