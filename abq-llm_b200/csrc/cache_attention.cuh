@@ -10,7 +10,12 @@
 // lengths, each with a ring of bulk copies of its own (a granule is one contiguous copy), queries straight from global memory to registers, no barrier of the
 // block anywhere.  An item (sequence, head, row block) counts for kCaExtra granules more than it has: its queries and its result cost about that much
 // (without it, runs over many short sequences took twice as long as those over long ones).  Pieces of an item that several warps hold meet in the
-// workspace, added by a second kernel in order (no atomics).
+// workspace, added by a second kernel in order (no atomics): joined by whichever warp comes last they took twice the time of both kernels, since one warp has
+// too few loads under way.
+//
+// Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 106 (76.7, so 72 % of the rate); 32 of
+// up to 2000 tokens, 4 bits 21.9 (4.8); one of 1024 tokens, 32 heads 10.1 (1.3): 3 us until a warp has found its run and its first copy is there, and 4 us for
+// the second kernel, are what short calls cost.
 //
 //  * Running maximum: raised only when a score passes it by more than 2^8 (checked with one vote), so that shuffles and the scaling of O are rare.
 //  * p vs_j is rounded to fp16 after scaling by a power of two that keeps the largest vs seen so far near 2^6: with p <= 2^8 the product is below 2^15 and
