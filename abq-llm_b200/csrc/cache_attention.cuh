@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attentio
         mbar_init(&full[lane], 1);
     fence_mbar_init();
     __syncwarp();
-    pdl_launch_dependents();
     pdl_wait_prior_grid();
+    pdl_launch_dependents();
 
     const int run = blockIdx.x * kCaWarps + warp;
     CaRun line;
@@ -650,8 +650,6 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
 {
     constexpr int kLanes = D / 8, kGroups = kCaThreads / kLanes;
     __shared__ float sums[kCaThreads][9];
-    pdl_launch_dependents();
-    pdl_wait_prior_grid();
     const int items = a.kv_heads * a.row_blocks, b = blockIdx.x / items, item = blockIdx.x - b * items;
     long long units, prefix;
     ca_sums(a, b, units, prefix);
@@ -662,9 +660,11 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
     if (G) {
         c0 = (int)ca_div(start + a.extra, quota);
         c1 = (int)ca_div(start + a.extra + G - 1, quota);
-        if (c0 == c1)
-            return;
     }
+    pdl_wait_prior_grid();
+    pdl_launch_dependents();
+    if (G && c0 == c1)
+        return;
     const int head = item / a.row_blocks, row0 = (item - head * a.row_blocks) * tile_rows, rows = min(a.n * a.group - row0, tile_rows);
     const int sub = threadIdx.x % kLanes, grp = threadIdx.x / kLanes, row = blockIdx.y * row_groups + grp % row_groups, turn = grp / row_groups, turns = kGroups / row_groups;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part + 2 * (size_t)a.runs * a.slot_rows * D);

@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
     // exist twice and their next phase but one follows p_ready of the tile between; o_done, p_ready and q_ready follow one another; k_free and
     // slot_free are waited for by the warps whose next arrival their next phase needs.
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = blockIdx.x;
-    pdl_launch_dependents();
     pdl_wait_prior_grid();
+    pdl_launch_dependents();
     CaRun line;
     if (!line.begin(a, run, lane))
         return; // the whole block
