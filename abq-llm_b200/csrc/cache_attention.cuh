@@ -671,21 +671,9 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
     float v[8] = {}, lsum = 0.f;
     if (row < rows && G) {
         auto slot_of = [&](int c) { return 2 * (size_t)c + (c == c0 && c0 * quota < start ? 1 : 0); };
-        float top = -INFINITY;
-        for (int c = c0 + sub; c <= c1; c += 4 * kLanes) {
-            float x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                x[u] = c + u * kLanes <= c1 ? ml[slot_of(c + u * kLanes) * a.slot_rows + row].x : -INFINITY;
-            top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-        }
-        const unsigned lanes = kLanes == 16 ? 0xffffu << (threadIdx.x & 16) : 0xffu << (threadIdx.x & 24);
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1)
-            top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
-        for (int c = c0 + turn; c <= c1; c += 4 * turns) { // four pieces under way
-            float2 p[4];
-            float4 lo[4], hi[4];
+        float2 p[4];
+        float4 lo[4], hi[4];
+        auto fetch = [&](int c) { // four pieces under way
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int at = c + u * turns;
@@ -699,6 +687,21 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
                     hi[u] = *reinterpret_cast<const float4 *>(src + 4);
                 }
             }
+        };
+        fetch(c0 + turn); // (used behind the maximum)
+        float top = -INFINITY;
+        for (int c = c0 + sub; c <= c1; c += 4 * kLanes) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                x[u] = c + u * kLanes <= c1 ? ml[slot_of(c + u * kLanes) * a.slot_rows + row].x : -INFINITY;
+            top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        }
+        const unsigned lanes = kLanes == 16 ? 0xffffu << (threadIdx.x & 16) : 0xffu << (threadIdx.x & 24);
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1)
+            top = fmaxf(top, __shfl_xor_sync(lanes, top, o));
+        for (int c = c0 + turn; c <= c1;) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const float f = p[u].x == -INFINITY ? 1.f : ex2(p[u].x - top);
@@ -706,6 +709,9 @@ __global__ void __launch_bounds__(kCaThreads) cache_attention_combine_kernel(con
                 v[0] = fmaf(f, lo[u].x, v[0]), v[1] = fmaf(f, lo[u].y, v[1]), v[2] = fmaf(f, lo[u].z, v[2]), v[3] = fmaf(f, lo[u].w, v[3]);
                 v[4] = fmaf(f, hi[u].x, v[4]), v[5] = fmaf(f, hi[u].y, v[5]), v[6] = fmaf(f, hi[u].z, v[6]), v[7] = fmaf(f, hi[u].w, v[7]);
             }
+            c += 4 * turns;
+            if (c <= c1)
+                fetch(c);
         }
     }
     if (turns > 1) {
