@@ -22,13 +22,13 @@ struct CaPlan {
     int block, most_runs;   // rows of a block; runs the line is cut into at most
     int unit_log2, extra, min_quota;
 };
-static CaPlan ca_plan(int rows)
+static CaPlan ca_plan(int rows, int head_dim)
 {
     const int blocks = (rows + 127) / 128;
     if (rows >= 96 && 4 * rows >= 3 * 128 * blocks) // (measured: see there)
         return { true, 128, kCaSms, 7, 1, 2 };
     const int tiles = row_tiles(rows);
-    return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(tiles) * kCaWarps, 4, kCaExtra, kCaMinQuota };
+    return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(head_dim, tiles) * kCaWarps, 4, kCaExtra, kCaMinQuota };
 }
 
 static bool attention_shape_valid(const abq_kv_cache &c, int batch, int n, int q_heads)
@@ -46,7 +46,7 @@ extern "C" size_t abq_cache_attention_workspace_bytes(const abq_kv_cache *cache,
     if (!cache || !attention_shape_valid(*cache, batch, rows_per_seq, q_heads))
         return 0;
     const int rows = rows_per_seq * (q_heads / cache->kv_heads);
-    const CaPlan plan = ca_plan(rows);
+    const CaPlan plan = ca_plan(rows, cache->head_dim);
     return (size_t)2 * plan.most_runs * std::min(rows, plan.block) * (cache->head_dim + 2) * sizeof(float);
 }
 
@@ -77,7 +77,7 @@ extern "C" abq_status abq_cache_attention(const abq_cache_attention_params *p, a
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.page_magic = ((1ull << 34) + a.page_granules - 1) / a.page_granules;
     const int rows = a.n * a.group;
-    const CaPlan plan = ca_plan(rows);
+    const CaPlan plan = ca_plan(rows, p->cache.head_dim);
     a.row_blocks = (rows + plan.block - 1) / plan.block;
     a.slot_rows = std::min(rows, plan.block);
     a.unit_log2 = plan.unit_log2, a.extra = plan.extra, a.min_quota = plan.min_quota;

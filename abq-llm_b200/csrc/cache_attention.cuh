@@ -13,8 +13,8 @@
 // workspace, added by a second kernel in order (no atomics): joined by whichever warp comes last they took twice the time of both kernels, since one warp has
 // too few loads under way.
 //
-// Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 106 (76.7, so 72 % of the rate); 32 of
-// up to 2000 tokens, 4 bits 21.9 (4.8); one of 1024 tokens, 32 heads 10.1 (1.3): 3 us until a warp has found its run and its first copy is there, and 4 us for
+// Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 95 (76.7, so 81 % of the rate); 32 of
+// up to 4096 tokens, 4 bits 20.7 (4.8); one of 1024 tokens, 32 heads 8.9 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for
 // the second kernel, are what short calls cost.
 //
 //  * Running maximum: raised only when a score passes it by more than 2^8 (checked with one vote), so that shuffles and the scaling of O are rare.
@@ -38,7 +38,9 @@ constexpr int kCaSms = 148;
 constexpr int kCaMinQuota = 4; // granules a warp takes at least
 constexpr int kCaExtra = 2;    // what an item costs beside its granules, in granules
 
-__host__ __device__ constexpr int ca_ctas_per_sm(int tiles) { return tiles == 1 ? 3 : 2; } // 168 or 255 registers a thread
+// 128, 168 or 255 registers a thread: as many CTAs as fit without spills (heads of 64 with one more than heads of 128: two sequences of 64 K tokens, 40 heads, one
+// row 137 us instead of 149, 26 rows over 4 of up to 2049 27 instead of 29; heads of 128 with spills for one more 45 instead of 35)
+__host__ __device__ constexpr int ca_ctas_per_sm(int head_dim, int tiles) { return (tiles == 1 ? 3 : 2) + (head_dim == 64); }
 
 struct CacheAttnArgs {
     const uint8_t *data;
@@ -226,7 +228,7 @@ template <int D, int BITS, int NT>
 struct CaShape {
     static constexpr int RB = kv_row_bytes(D, BITS), kGranule = kv_granule_bytes(RB), kRows = 8 * NT, kSteps = D / 16;
     static constexpr int kFixed = kCaWarps * kRows * 8;
-    static constexpr int kRoom = 226 * 1024 / ca_ctas_per_sm(NT) - 1024 - kFixed;
+    static constexpr int kRoom = 226 * 1024 / ca_ctas_per_sm(D, NT) - 1024 - kFixed;
     static constexpr int kFit = kRoom / (kCaWarps * (kGranule + 8));
     static constexpr int kStages = kFit < 10 ? kFit : 10;
     static constexpr int kSmem = kFixed + kCaWarps * kStages * (kGranule + 8);
@@ -234,7 +236,7 @@ struct CaShape {
 };
 
 template <int D, int BITS, int NT, bool BF16>
-__global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(NT)) cache_attention_kernel(const __grid_constant__ CacheAttnArgs a)
+__global__ void __launch_bounds__(kCaThreads, ca_ctas_per_sm(D, NT)) cache_attention_kernel(const __grid_constant__ CacheAttnArgs a)
 {
     using Sh = CaShape<D, BITS, NT>;
     constexpr int RB = Sh::RB, kGranule = Sh::kGranule, kRows = Sh::kRows, kSteps = Sh::kSteps, kStages = Sh::kStages, kTiles = D / 16;
