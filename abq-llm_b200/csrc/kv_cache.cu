@@ -73,33 +73,41 @@ __device__ __forceinline__ uint64_t fma_floats(uint64_t a, uint64_t b, uint64_t 
     return r;
 }
 
-template <int D, int BITS, bool BF16>
-__device__ __forceinline__ void quantise_row(const uint4 &x, int sub, int place, uint8_t *granule, int part, bool kept)
+// (min, -max) of a lane's eight values
+template <bool BF16>
+__device__ __forceinline__ uint32_t range8(const uint4 &x)
 {
-    constexpr int RB = kv_row_bytes(D, BITS), kLanes = D / 8;
-    const uint32_t w[4] = { x.x, x.y, x.z, x.w };
-    const uint32_t lo = pair_min<BF16>(pair_min<BF16>(w[0], w[1]), pair_min<BF16>(w[2], w[3]));
-    const uint32_t hi = pair_max<BF16>(pair_max<BF16>(w[0], w[1]), pair_max<BF16>(w[2], w[3])) ^ 0x80008000u;
-    uint32_t range = pair_min<BF16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632)); // (min, -max)
-#pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1)
-        range = pair_min<BF16>(range, __shfl_xor_sync(0xffffffffu, range, o));
+    const uint32_t lo = pair_min<BF16>(pair_min<BF16>(x.x, x.y), pair_min<BF16>(x.z, x.w));
+    const uint32_t hi = pair_max<BF16>(pair_max<BF16>(x.x, x.y), pair_max<BF16>(x.z, x.w)) ^ 0x80008000u;
+    return pair_min<BF16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+}
+
+// A row's parameters from its range: the 32 bits (scale, min) that are stored, and the scale's reciprocal, or 0 where that is no use (a scale of 0, or one whose
+// reciprocal is not a normal number)
+template <int BITS, bool BF16>
+__device__ __forceinline__ uint32_t row_params(uint32_t range, float &inv)
+{
     const float2 mm = half_pair_to_float(range, BF16);
-    const float mn = mm.x, spread = -mm.y - mm.x;
-    const bool finite = spread <= 3.402823466e38f; // (not for Inf or NaN among the values)
-    const float fine = spread / (float)((1 << BITS) - 1);
+    const float spread = -mm.y - mm.x, fine = spread / (float)((1 << BITS) - 1);
     uint32_t sbits = float_pair_to_half(fine, 0.f, BF16) & 0xffffu;
     if (half_bits_to_float(sbits, BF16) < fine)
         ++sbits; // up to the next 16-bit value (positive values are ordered like their bits)
     const float s = half_bits_to_float(sbits, BF16);
-    float inv;
     asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s)); // at most 1 ulp off
-    const bool usual = s >= 1.17549435e-38f && s <= 8.5e37f; // the reciprocal is a normal number
-    inv = usual ? inv : 0.f;
+    inv = s >= 1.17549435e-38f && s <= 8.5e37f ? inv : 0.f;
+    return spread <= 3.402823466e38f ? sbits | range << 16 : BF16 ? 0x7fc07fc0u : 0x7e007e00u; // (not for Inf or NaN among the values)
+}
+
+template <int D, int BITS, bool BF16>
+__device__ __forceinline__ void quantise_row(const uint4 &x, uint32_t params, float inv, int at, uint8_t *rows, bool kept)
+{
+    const uint32_t w[4] = { x.x, x.y, x.z, x.w };
+    const float2 sm = half_pair_to_float(params, BF16);
+    const float s = sm.x, mn = sm.y;
     const float less = inv * (1.f - 9.5367432e-7f), more = inv * (1.f + 9.5367432e-7f);
     const uint64_t less2 = pack_floats(less, less), more2 = pack_floats(more, more), mn2 = pack_floats(-mn, -mn);
     const uint64_t magic2 = pack_floats(12582912.f, 12582912.f); // 1.5 * 2^23: the sum's low bits are the rounded value
-    uint32_t code[8], differ = s > 0.f && !usual;
+    uint32_t code[8], differ = s > 0.f && inv == 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = half_pair_to_float(w[i], BF16);
@@ -117,32 +125,49 @@ __device__ __forceinline__ void quantise_row(const uint4 &x, int sub, int place,
             code[2 * i + 1] = s > 0.f ? (uint32_t)__float2int_rn((f.y - mn) / s) : 0u;
         }
     }
-    if (!finite) {
+    if (s != s) { // NaN stands for the row
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             code[i] = 0;
     }
     if (!kept)
         return;
-    uint8_t *rows = granule + part * 16 * RB;
-    const int t = place & 15;
     if (BITS == 8) {
         uint2 o;
         o.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
         o.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
-        *reinterpret_cast<uint2 *>(rows + kv_place<RB>(t, sub * 8)) = o;
+        *reinterpret_cast<uint2 *>(rows + at) = o;
     } else {
         uint32_t two[4]; // the low byte: two codes
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             two[i] = code[2 * i] + (code[2 * i + 1] << 4);
         const uint32_t o = __byte_perm(__byte_perm(two[0], two[1], 0x0040), __byte_perm(two[2], two[3], 0x0040), 0x5410);
-        *reinterpret_cast<uint32_t *>(rows + kv_place<RB>(t, sub * 4)) = o;
+        *reinterpret_cast<uint32_t *>(rows + at) = o;
     }
-    if (sub == 0) {
-        const uint32_t pair = finite ? sbits | range << 16 : (BF16 ? 0x7fc07fc0u : 0x7e007e00u);
-        *reinterpret_cast<uint32_t *>(granule + kv_param_offset(RB, part) + 4 * t) = pair;
-    }
+}
+
+// A token's rows of keys and values of one head.  The lower half of the lanes takes the keys' range and parameters, the upper half the values': what is the same for a
+// whole row is worked out by half as many instructions.
+template <int D, int BITS, bool BF16>
+__device__ __forceinline__ void quantise_token(const uint4 &x, const uint4 &y, int sub, int place, uint8_t *granule, bool kept)
+{
+    constexpr int RB = kv_row_bytes(D, BITS), kLanes = D / 8, kHalf = kLanes / 2;
+    const bool upper = sub >= kHalf;
+    const uint32_t rx = range8<BF16>(x), ry = range8<BF16>(y);
+    uint32_t range = pair_min<BF16>(upper ? ry : rx, __shfl_xor_sync(0xffffffffu, upper ? rx : ry, kHalf));
+#pragma unroll
+    for (int o = 1; o < kHalf; o <<= 1)
+        range = pair_min<BF16>(range, __shfl_xor_sync(0xffffffffu, range, o));
+    float inv;
+    const uint32_t params = row_params<BITS, BF16>(range, inv);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, params, kHalf);
+    const float other_inv = __shfl_xor_sync(0xffffffffu, inv, kHalf);
+    const int t = place & 15, at = kv_place<RB>(t, sub * BITS);
+    quantise_row<D, BITS, BF16>(x, upper ? other : params, upper ? other_inv : inv, at, granule, kept);
+    quantise_row<D, BITS, BF16>(y, upper ? params : other, upper ? inv : other_inv, at, granule + 16 * RB, kept);
+    if (kept && (sub & (kHalf - 1)) == 0)
+        *reinterpret_cast<uint32_t *>(granule + (upper ? kv_param_offset(RB, 1) : kv_param_offset(RB, 0)) + 4 * t) = params;
 }
 
 struct KvWriteArgs {
@@ -173,15 +198,15 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteArgs 
         x = *reinterpret_cast<const uint4 *>(ks + h0 * a.k_head_stride);
         y = *reinterpret_cast<const uint4 *>(vs + h0 * a.v_head_stride);
     }
-    for (int h = h0; h < h1; ++h) {
+    uint8_t *granule = kv_granule(a.c, page, place, h0, kGranule);
+    const size_t head_step = (size_t)(a.c.page_size >> 4) * kGranule;
+    for (int h = h0; h < h1; ++h, granule += head_step) {
         uint4 nx = x, ny = y; // the next head's rows are under way while this one's are quantised
         if (kept && h + 1 < h1) {
             nx = *reinterpret_cast<const uint4 *>(ks + (h + 1) * a.k_head_stride);
             ny = *reinterpret_cast<const uint4 *>(vs + (h + 1) * a.v_head_stride);
         }
-        uint8_t *granule = kv_granule(a.c, page, place, h, kGranule);
-        quantise_row<D, BITS, BF16>(x, sub, place, granule, 0, kept);
-        quantise_row<D, BITS, BF16>(y, sub, place, granule, 1, kept);
+        quantise_token<D, BITS, BF16>(x, y, sub, place, granule, kept);
         x = nx;
         y = ny;
     }
