@@ -25,7 +25,7 @@ struct CaPlan {
 static CaPlan ca_plan(int rows, int head_dim)
 {
     const int blocks = (rows + 127) / 128;
-    if (rows >= 96 && 4 * rows >= 3 * 128 * blocks) // (measured: see there)
+    if (rows >= 80 * blocks) // (measured: see there)
         return { true, 128, kCaSms, 7, 1, 2 };
     const int tiles = row_tiles(rows);
     return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(head_dim, tiles) * kCaWarps, 4, kCaExtra, kCaMinQuota };

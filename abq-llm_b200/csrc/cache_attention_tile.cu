@@ -5,15 +5,18 @@
 // swizzled operand tiles in shared memory.  Scale and offset of a token's key and value are applied to its column of S and of p.
 //
 // Roles of a CTA (one per SM; each takes an equal run of the line of tiles of all sequences, heads and row blocks):
-//   warps 0-3   softmax, a thread per lane; they also put the queries into shared memory and write the result
-//   warps 4-11  expand codes, a granule each of a tile
-//   warp 12     issues the products (S of the next tile before P of this one: S is double-buffered)
-//   warp 13     bulk copies of granules, two tiles ahead
-// What bounds it: the softmax, about 24 clocks a score and lane: four parameters per token come to every row from shared memory, whose return path (16 bytes a
-// thread) is as busy as the multiply-add pipes.  3100 clocks a tile of 128 tokens; expanding it takes 1400, its products 512 (D = 64) or 1024.
-// Measured against blocks of 16 rows on mma.sync (us; 8 bits, heads of 128): 256 rows over 4 sequences of up to 2000 tokens and 8 heads 40.0 and 50.8, over one of 8000
-// 44.5 and 68.7, over 32 of up to 300 83.0 and 91.4; 96 rows 29.1 and 29.1, 30.1 and 35.0, 44.4 and 40.2; 64 rows 27.4 and 24.1, 25.6 and 27.8, 43.5 and 30.5.
-// So it is taken from 96 rows on, and where a last block is at least three quarters full (160 rows over the 32 short ones: 80.0 and 59.0).
+//   warps 0-7   softmax: a row has two threads, of 64 of the tile's tokens each.  They agree on the maximum where one has to look for it and share the rest at the
+//               end; each loads half of the row's queries, scales and writes half of its result
+//   warps 8-15  expand codes, a granule each of a tile
+//   warp 16     issues the products (S of the next tile before P of this one: S is double-buffered)
+//   warp 17     bulk copies of granules, two tiles ahead
+// What bounds it: softmax and expansion alike.  Four parameters per token come to every row from shared memory, whose return path takes 2048 clocks a tile for that;
+// with one thread a row the softmax took 3100 (latency: 16 trees of 64 rows, heads of 64, 36 us instead of 31; four of 2000 tokens, heads of 128, 45 instead
+// of 42).  Expanding a tile takes 1400, its products 512 (D = 64) or 1024.
+// Measured against blocks of 16 rows on mma.sync (us; 8 bits, heads of 128, 8 key heads): rows over 4 sequences of up to 2000 tokens, over one of 8000, over 32 of up to
+// 300: 64 rows 20.6 and 21.9, 21.8 and 25.9, 31.0 and 29.8; 80 rows 22.2 and 24.8, 22.8 and 29.7, 32.5 and 33.0; 96 rows 23.4 and 26.2, 23.3 and 32.8, 34.3 and
+// 39.9; 160 rows 30.8 and 32.9, 33.6 and 46.3, 61.0 and 58.4; heads of 64 and 4 bits, 64 rows 18.2 and 18.0, 20.7 and 21.5, 26.6 and 21.5; 80 rows 18.7 and 19.8, 21.0
+// and 24.4, 27.0 and 23.6.  So it is taken where its blocks are at least five eighths full.
 //
 // The maximum is looked for at a run's first tile and where the sum over a tile says that it has risen by more than 2^8; the value scales' power of two as in
 // cache_attention.cuh, but as a part of the exponent: p is 2^(s - m) 2^(6 - L) throughout (L at least -60, so that no sum of p overflows).
@@ -25,16 +28,16 @@
 
 namespace abq {
 
-constexpr int kCtThreads = 512;
+constexpr int kCtThreads = 640; // (18 warps have work; registers are dealt out by fours of warps)
 constexpr int kCtKeys = 128;
 
 template <int D, int BITS>
 struct CtShape {
     static constexpr int RB = kv_row_bytes(D, BITS), kGranule = kv_granule_bytes(RB), kRaw = 8 * kGranule;
     static constexpr int kTile = kCtKeys * D * 2, kHalf = 128 * 128, kHalves = D / 64;
-    static constexpr int kPar = 2 * 128 * 16;
-    // queries, keys, two of values, two raw tiles, token parameters, 1024 to align, the rest
-    static constexpr int kSmem = 4 * kTile + 2 * kRaw + kPar + 1024 + 1024;
+    static constexpr int kPar = 2 * 128 * 16, kMeet = 2 * 2 * 128 * 8;
+    // queries, keys, two of values, two raw tiles, token parameters, what halves of a row tell each other, 1024 to align, the rest
+    static constexpr int kSmem = 4 * kTile + 2 * kRaw + kPar + kMeet + 1024 + 1024;
     static constexpr int kP = 256, kO = 384; // TMEM columns: S at 0 and 128
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -51,10 +54,11 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t *sq = smem, *sk = smem + kTile, *sv = smem + 2 * kTile, *raw = smem + 4 * kTile;
     float4 *par = reinterpret_cast<float4 *>(raw + 2 * Sh::kRaw); // [2][128]: key scale and offset, value scale and offset
-    uint64_t *bars = reinterpret_cast<uint64_t *>(raw + 2 * Sh::kRaw + Sh::kPar);
+    float2 *slots = reinterpret_cast<float2 *>(raw + 2 * Sh::kRaw + Sh::kPar); // [2][2 halves][128 rows]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(raw + 2 * Sh::kRaw + Sh::kPar + Sh::kMeet);
     uint64_t *raw_full = bars, *raw_empty = bars + 2, *ready = bars + 4, *k_free = bars + 6, *slot_free = bars + 7, *s_full = bars + 9, *s_read = bars + 11,
-             *p_ready = bars + 13, *o_done = bars + 14, *q_ready = bars + 15, *drain = bars + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 18);
+             *p_ready = bars + 13, *o_done = bars + 14, *q_ready = bars + 15, *drain = bars + 16, *pair = bars + 17;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 22);
     uint32_t *raw_good = tmem_slot + 2;                                  // [2] which granules of a raw tile lie in the cache
     float *vmaxs = reinterpret_cast<float *>(tmem_slot + 4);             // [2][8] largest value scale of each granule
     uint8_t *gbad = reinterpret_cast<uint8_t *>(vmaxs + 16);             // [2][8] granules that are not in the cache
@@ -75,16 +79,18 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             mbar_init(&ready[i], 8);
             mbar_init(&slot_free[i], 1);
             mbar_init(&s_full[i], 1);
-            mbar_init(&s_read[i], 4);
+            mbar_init(&s_read[i], 8);
         }
         mbar_init(k_free, 1);
-        mbar_init(p_ready, 4);
+        mbar_init(p_ready, 8);
         mbar_init(o_done, 1);
-        mbar_init(q_ready, 4);
+        mbar_init(q_ready, 8);
+        for (int i = 0; i < 4; ++i)
+            mbar_init(&pair[i], 2);
         mbar_init(drain, 1);
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -96,15 +102,28 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
     bool ok = true;
     CaPiece p;
 
-    if (warp < 4) {
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;"); // of 96 at launch: 2 * 128 + 2 * 72 + 80 = 5 * 96
         // ---------------------------------------------------------------- queries, softmax, result
-        const int row = warp * 32 + lane;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16, tp = tmem + lanes + (uint32_t)Sh::kP, to = tmem + lanes + (uint32_t)Sh::kO;
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tp = tmem + lanes + (uint32_t)Sh::kP, to = tmem + lanes + (uint32_t)Sh::kO;
         const int rows = a.n * a.group;
         float rf = 0.f, rs = 0.f; // score = S ks rf + ko rs
         uint64_t mask = 0;
         int at = 0, ctx = 0, len = 0;
-        auto load_queries = [&](const CaPiece &w) {
+        // what the two threads of a row tell each other; both come to every meeting, in the same order.  (Slots alternate: the other one may be at the next meeting.)
+        uint32_t met = 0;
+        auto meet = [&](float2 mine, float2 &theirs) {
+            float2 *at_meeting = slots + (met & 1) * 256;
+            at_meeting[half * 128 + row] = mine;
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&pair[warp & 3]);
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pair[warp & 3], met & 1, a.status, STATUS_TIMEOUT_PIPE)) && ok;
+            theirs = at_meeting[(half ^ 1) * 128 + row];
+            ++met;
+        };
+        auto load_queries = [&](const CaPiece &w) { // half a row each
             const int head = w.item / a.row_blocks;
             at = (w.item - head * a.row_blocks) * 128 + row;
             const bool live = at < rows;
@@ -114,23 +133,26 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             ctx = len - a.n;
             mask = !live ? 0 : a.tree ? a.tree[(size_t)w.b * a.n + i] : i >= 63 ? ~0ull : (2ull << i) - 1;
             float down = 1.f, back = 1.f, sum = 0.f;
-            uint4 v[D / 8]; // (all loads under way at once)
+            uint4 v[D / 16]; // (all loads under way at once)
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x)
-                v[x] = live ? *reinterpret_cast<const uint4 *>(src + x * 16) : make_uint4(0, 0, 0, 0);
+            for (int x = 0; x < D / 16; ++x)
+                v[x] = live ? *reinterpret_cast<const uint4 *>(src + half * D + x * 16) : make_uint4(0, 0, 0, 0);
+            float2 other;
             if (BF16) { // to [1, 2) by a power of two
                 uint32_t top = 0;
 #pragma unroll
-                for (int x = 0; x < D / 8; ++x)
+                for (int x = 0; x < D / 16; ++x)
                     top = __vmaxu2(__vmaxu2(top, v[x].x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v[x].y & 0x7fff7fffu, v[x].z & 0x7fff7fffu), v[x].w & 0x7fff7fffu));
                 top = max(top & 0xffffu, top >> 16);
+                meet(make_float2(__uint_as_float(top), 0.f), other);
+                top = max(top, __float_as_uint(other.x));
                 int e = (int)(top >> 7) - 127;
                 e = e > 127 || top == 0 ? 0 : max(e, -126);
                 down = __int_as_float(e == 127 ? 0x00400000 : (127 - e) << 23);
                 back = __int_as_float((127 + e) << 23);
             }
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x) {
+            for (int x = 0; x < D / 16; ++x) {
                 uint32_t w4[4] = { v[x].x, v[x].y, v[x].z, v[x].w };
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
@@ -141,8 +163,11 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                     const float2 f = half_pair_to_float(w4[y], false);
                     sum += f.x + f.y;
                 }
-                *reinterpret_cast<uint4 *>(sq + (x >> 3) * kHalf + row * 128 + (((x & 7) ^ (row & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+                const int chunk = half * (D / 16) + x;
+                *reinterpret_cast<uint4 *>(sq + (chunk >> 3) * kHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
             }
+            meet(make_float2(sum, 0.f), other);
+            sum += other.x;
             rf = a.scale_log2 * back;
             rs = sum * rf;
             fence_proxy_async();
@@ -155,7 +180,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             load_queries(p);
         while (more && ok) {
             const bool live = at < rows, some = __any_sync(0xffffffffu, live); // (of a warp of rows that do not exist nothing is read)
-            float m = -INFINITY, mm = 0.f, l = 0.f, bias = 0.f;                // mm = m + L - 6
+            float m = live ? -INFINITY : 0.f, mm = 0.f, l = 0.f, bias = 0.f;   // mm = m + L - 6 (no row: nothing to look for)
             float vmax = 0.f;                                                  // 2^(L + 1)
             int L = -121;
             const int tiles = p.g1 - p.g0;
@@ -188,7 +213,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                     auto weights = [&](auto masked) {
                         tl = tb = 0.f;
 #pragma unroll 1
-                        for (int x0 = 0; x0 < kCtKeys; x0 += 16) {
+                        for (int x0 = half * (kCtKeys / 2); x0 < (half + 1) * (kCtKeys / 2); x0 += 16) {
                             float s[16];
                             float4 k[2][4];
 #pragma unroll
@@ -224,7 +249,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                         if (look) {
                             float top = -INFINITY;
 #pragma unroll 1
-                            for (int x0 = 0; x0 < kCtKeys; x0 += 16) {
+                            for (int x0 = half * (kCtKeys / 2); x0 < (half + 1) * (kCtKeys / 2); x0 += 16) {
                                 float s[16];
                                 pa_ld16(ts + x0, s);
                                 const uint32_t vis = seen(x0);
@@ -241,9 +266,13 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                                     }
                                 }
                             }
+                            float2 other;
+                            meet(make_float2(top, 0.f), other);
+                            top = pa_max3(top, other.x, other.x);
                             if (!(top < INFINITY)) // NaN (or an overflow): the row's result
                                 l = NAN;
                             const float before = mm;
+                            const bool first = m == -INFINITY; // (before the first score of a row its sums are 0, whatever they are multiplied by)
                             if (top > m + 8.f)
                                 m = top;
                             if (vtop >= vmax) {
@@ -251,14 +280,13 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                                 vmax = __int_as_float(min(128 + L, 255) << 23);
                             }
                             mm = m == -INFINITY ? 0.f : m + (float)(L - 6);
-                            // (before the first score of a row its sums are 0, whatever they are multiplied by)
-                            const float f = l == 0.f ? 1.f : pa_ex2(before - mm);
+                            const float f = first ? 1.f : pa_ex2(before - mm);
                             if (__any_sync(0xffffffffu, f != 1.f)) {
                                 l *= f;
                                 bias *= f;
                                 if (j > 0) {
 #pragma unroll 1
-                                    for (int x = 0; x < D; x += 32) {
+                                    for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
                                         float o[32];
                                         pa_ld32(to + x, o);
                                         pa_ld_wait(o);
@@ -277,14 +305,21 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                         else
                             weights(std::false_type());
                         // no p above 2^8 (in units of 2^(6 - L)), so none times a value scale above 2^15
-                        if (look || __all_sync(0xffffffffu, tl <= __int_as_float((127 + 14 - L) << 23)))
+                        if (look)
                             break;
-                        look = true;
+                        look = !__all_sync(0xffffffffu, tl <= __int_as_float((127 + 14 - L) << 23));
+                        float2 other;
+                        meet(make_float2(look ? 1.f : 0.f, 0.f), other);
+                        look = look || other.x != 0.f;
+                        if (!look || !ok)
+                            break;
                     }
                     l += tl;
                     bias += tb;
                     pa_st_wait();
                 }
+                if (!ok) // (a meeting that did not take place)
+                    break;
                 tmem_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -299,7 +334,13 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             more = line.next(a, p);
             if (more)
                 load_queries(p);
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(o_done, (T - 1) & 1, a.status, STATUS_TIMEOUT_MMA));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(o_done, (T - 1) & 1, a.status, STATUS_TIMEOUT_MMA));
+            float2 other;
+            if (!ok)
+                break;
+            meet(make_float2(l, bias), other);
+            l += other.x;
+            bias += other.y;
             if (!ok)
                 break;
             tmem_fence_after();
@@ -326,7 +367,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             const int to_row = row0 + row;
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-            for (int x = 0; x < D; x += 16) {
+            for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 16) {
                 float o[16];
                 pa_ld16(to + x, o);
                 if (to_row < rows) {
@@ -339,13 +380,14 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                     put(to_row, x + 8, o + 8, inv);
                 }
             }
-            if (!whole && to_row < rows)
+            if (half == 0 && !whole && to_row < rows)
                 ml[row] = make_float2(l == 0.f ? -INFINITY : mm, l);
             tmem_fence_before(); // (O is read before the next piece's first product, which waits for this warp's p)
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ---------------------------------------------------------------- codes -> operand tiles
-        const int w = warp - 4, t = lane & 15, h = lane >> 4, key = 16 * w + t;
+        const int w = warp - 8, t = lane & 15, h = lane >> 4, key = 16 * w + t;
         constexpr int kBytes = RB / 2; // of a lane: half a row of keys, half a row of values
         auto expand = [&](const uint8_t *src, uint8_t *dst) {
 #pragma unroll
@@ -400,7 +442,10 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                 }
             }
         }
-    } else if (warp == 12) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    }
+    if (warp == 16) {
         // ---------------------------------------------------------------- products
         uint32_t pieces = 0;
         while (ok && line.next(a, p)) {
@@ -453,7 +498,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             mbar_wait_bounded(drain, 0, a.status, STATUS_TIMEOUT_MMA);
         }
         __syncwarp();
-    } else if (warp == 13) {
+    } else if (warp == 17) {
         // ---------------------------------------------------------------- copies
         while (ok && line.next(a, p)) {
             const int granules = (int)(((long long)ca_tokens(a, p.b) + 15) >> 4), head = p.item / a.row_blocks;
@@ -490,7 +535,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
 
     tmem_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }

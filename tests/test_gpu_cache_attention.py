@@ -239,3 +239,20 @@ def test_offsets_beyond_32_bits(abq, cuda):
     assert bool(((out.cpu().double() - want).abs() <= bound).all())
     codes, scale, low = R.quantise(k, bits)
     assert torch.equal(ko.cpu(), (codes.float() * scale.float() + low.float()).half())
+
+
+@pytest.mark.parametrize("group,n", [(79, 1), (5, 16), (53, 3), (40, 4)])
+def test_rows_around_the_choice_of_kernel(abq, cuda, group, n):
+    s = Setup(abq, dim=64, bits=8, half=torch.float16, heads=2 * group, kv_heads=2, n=n, lens=[500, 61, n, 0], page=32, tree=True, seed=group).fill()
+    s.check(s.call())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_maximum_that_rises_in_either_half_of_a_tile(abq, cuda, dim):
+    """Tokens far above all before them, in the second half of a tile of 128, the first half of the next, the second again, and in both of one."""
+    s = Setup(abq, dim=dim, bits=8, half=torch.bfloat16, heads=4, kv_heads=1, n=32, lens=[1000], page=16, seed=dim)
+    s.q[:] = 1.0
+    for token, size in ((200, 3.0), (300, 6.0), (450, 9.0), (530, 12.0), (620, 12.5)):
+        s.k[token] = size
+    s.fill()
+    s.check(s.call())
