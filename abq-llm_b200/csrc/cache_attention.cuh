@@ -14,7 +14,7 @@
 // too few loads under way.
 //
 // Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 95 (76.7, so 81 % of the rate); 32 of
-// up to 4096 tokens, 4 bits 20.7 (4.8); one of 1024 tokens, 32 heads 8.9 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for
+// up to 4096 tokens, 4 bits 20.2 (4.8); one of 1024 tokens, 32 heads 8.9 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for
 // the second kernel, are what short calls cost.
 //
 //  * Running maximum: raised only when a score passes it by more than 2^8 (checked with one vote), so that shuffles and the scaling of O are rare.
@@ -36,7 +36,9 @@ constexpr int kCaWarps = 4;
 constexpr int kCaThreads = 32 * kCaWarps;
 constexpr int kCaSms = 148;
 constexpr int kCaMinQuota = 4; // granules a warp takes at least
-constexpr int kCaExtra = 2;    // what an item costs beside its granules, in granules
+// What an item costs beside its granules, in granules.  Measured with 1, 2, 3, 4, 5, 6 (us): 29 sequences of up to 4096 tokens, one row 21.5 20.7 20.0 20.2 19.9 19.9; 4 of up to
+// 2049, 26 rows 35.4 35.6 34.4 33.7 33.7 35.0; one of 1024, one row 9.9 8.9 9.1 9.0 8.9 9.0.
+constexpr int kCaExtra = 4;
 
 // 128, 168 or 255 registers a thread: as many CTAs as fit without spills (heads of 64 with one more than heads of 128: two sequences of 64 K tokens, 40 heads, one
 // row 137 us instead of 149, 26 rows over 4 of up to 2049 27 instead of 29; heads of 128 with spills for one more 45 instead of 35)
