@@ -184,25 +184,6 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream
 
 
-def _raw_stream(stream):
-    """As _stream(), without making a Stream object for the current one where torch has a way to (a call of a few microseconds shows the difference)."""
-    if stream is not None:
-        return _stream(stream)
-    global _current_raw
-    if _current_raw is None:
-        import torch
-        get, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
-        if get is None or device is None:
-            _current_raw = lambda: _stream(None)  # noqa: E731
-        else:
-            torch.cuda.current_stream()  # (initialises CUDA)
-            _current_raw = lambda: get(device())  # noqa: E731
-    return _current_raw()
-
-
-_current_raw = None
-
-
 def _check(status: int, what: str) -> None:
     if status != 0:
         extra = ""
@@ -384,23 +365,24 @@ def _one_device(**tensors) -> int:
     return next(iter(found.values()))
 
 
-_current_device = None
+_current_device = _current_raw = None  # index of the current device; address of a device's current stream
 
 
 def _launch(entry: str, params, stream) -> None:
-    """The call on the device its tensors are on, whichever is current; ``stream`` None: that device's current stream."""
-    global _current_device
+    """The call on the device its tensors are on, whichever is current; ``stream`` None: that device's current stream.  (Without making a Stream object for it
+    where torch has a way to: a call of a few microseconds shows the difference.)"""
+    global _current_device, _current_raw
     if _current_device is None:
         import torch
         torch.cuda.init()
+        _current_raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
         _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-    call = getattr(_lib or lib(), entry)
-    if params._device == _current_device():
-        status = call(ctypes.byref(params), _raw_stream(stream))
-    else:
+    device = params._device
+    if device != _current_device():
         import torch
-        with torch.cuda.device(params._device):
-            status = call(ctypes.byref(params), _raw_stream(stream))
+        with torch.cuda.device(device):
+            return _launch(entry, params, stream)
+    status = getattr(_lib or lib(), entry)(ctypes.byref(params), _current_raw(device) if stream is None else _stream(stream))
     if status:
         _check(status, entry)
 

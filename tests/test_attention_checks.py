@@ -138,7 +138,7 @@ def test_calls_go_to_the_device_of_their_tensors(abq, monkeypatch):
             now[0] = self.old
 
     monkeypatch.setattr(abq.binding, "_current_device", lambda: now[0])
-    monkeypatch.setattr(abq.binding, "_current_raw", lambda: 100 + now[0])
+    monkeypatch.setattr(abq.binding, "_current_raw", lambda index: 100 + index)
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(abq.binding, "_lib", NS(abq_kv_cache_write=lambda p, stream: seen.append((now[0], stream)) or 0))
     for device in (0, 1):
