@@ -10,8 +10,8 @@
 // close to the middle between two codes), or whose scale is below the normal range, is divided.  The scale is rounded up to 16 bits, so max never passes the
 // last code.
 //
-// Measured: 16001 tokens of 32 heads of 128, fp16 and 4 bits (332 MB either way): written in 90 us (3.7 TB/s; bound by instructions: 135 before the arithmetic was
-// packed and the divisions taken out), read back in 55 us (6.0 TB/s, 92 % of a copy's rate).
+// Measured: 16001 tokens of 32 heads of 128, fp16 and 4 bits (332 MB either way): written in 83 us (4.0 TB/s; bound by instructions: 135 before the arithmetic was
+// packed and the divisions taken out, 90 with every lane working out both rows' parameters), read back in 55 us (6.0 TB/s, 92 % of a copy's rate).
 #include <type_traits>
 
 #include "abq_kernels.h"
