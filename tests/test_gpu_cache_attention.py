@@ -256,3 +256,49 @@ def test_maximum_that_rises_in_either_half_of_a_tile(abq, cuda, dim):
         s.k[token] = size
     s.fill()
     s.check(s.call())
+
+
+@pytest.mark.parametrize("heads,kv_heads,n,lens", [(8, 2, 1, [0] * 45 + [70, 1, 0, 300] + [0] * 20), (4, 2, 3, [0, 0]), (8, 1, 12, [0] * 3), (16, 1, 8, [0] * 33 + [20])])
+def test_mostly_empty_batches(abq, cuda, heads, kv_heads, n, lens):
+    s = Setup(abq, dim=128, bits=4, half=torch.float16, heads=heads, kv_heads=kv_heads, n=n, lens=lens, page=16, tree=n > 1, seed=len(lens)).fill()
+    s.check(s.call())
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,n", [(8, 8, 1), (16, 2, 2), (16, 2, 10)])
+def test_lengths_that_change_between_calls_without_a_pause(abq, cuda, heads, kv_heads, n, captured):
+    """Each call and its second kernel see the lengths as they are at the call's place on the stream, however early the kernels are let in."""
+    s = Setup(abq, dim=128, bits=8, half=torch.float16, heads=heads, kv_heads=kv_heads, n=n, lens=[700, 45, 400], page=16, seed=13).fill()
+    s.call(run=False)
+    steps = torch.tensor([[-37, 0, -399], [30, -20, 350], [5, 19, -1], [2, 1, 50]] * 6, dtype=torch.int32, device="cuda")
+    outs = [torch.zeros((s.q.shape[0], heads, 128), dtype=torch.float16, device="cuda") for _ in steps]
+    cache = abq.make_kv_cache(s.held, page_size=16, kv_heads=kv_heads, head_dim=128, bits=8, dtype=torch.float16)
+    work = torch.empty(abq.cache_attention_workspace_bytes(cache, 3, n, heads), dtype=torch.uint8, device="cuda")
+    calls = [abq.make_cache_attention_params(cache, s.dq, o, s.dtable, s.dlens, scale=s.scale, workspace=work) for o in outs]
+    start = s.dlens.clone()
+
+    def run(pause):
+        s.dlens.copy_(start)
+        for step, call in zip(steps, calls):
+            s.dlens.add_(step).clamp_(0, 700)
+            abq.cache_attention(call)
+            abq.cache_attention(call)
+            if pause:
+                torch.cuda.synchronize()
+
+    run(True)
+    want = [o.clone() for o in outs]
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    if captured:
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run(False)
+        graph.replay()
+        graph.replay()
+    else:
+        run(False)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    assert not bool(want[0].isnan().any()) and bool(want[0].any())
