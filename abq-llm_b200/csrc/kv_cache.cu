@@ -185,19 +185,21 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteArgs 
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int sub = threadIdx.x % kLanes, token = blockIdx.x * kTokens + threadIdx.x / kLanes;
-    // lanes of rows that are left out stay for the shuffles, with a row of zeros that is not stored
-    const int64_t slot = token < a.tokens ? a.slots[token] : -1;
-    const bool kept = slot >= 0 && slot < a.c.capacity;
-    const int page = kept ? (int)(slot / a.c.page_size) : 0, place = kept ? (int)(slot - (int64_t)page * a.c.page_size) : 0;
+    // lanes of rows that are left out stay for the shuffles; what they work out is not stored
     const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(a.c.kv_heads, h0 + a.heads_per_cta);
-    const uint8_t *ks = a.k + (kept ? token * a.k_stride : 0) + sub * 16, *vs = a.v + (kept ? token * a.v_stride : 0) + sub * 16;
-    if (!__any_sync(0xffffffffu, kept))
-        return;
+    const bool exists = token < a.tokens;
+    const uint8_t *ks = a.k + (exists ? token * a.k_stride : 0) + sub * 16, *vs = a.v + (exists ? token * a.v_stride : 0) + sub * 16;
     uint4 x = make_uint4(0, 0, 0, 0), y = x;
-    if (kept) {
+    int64_t slot = -1;
+    if (exists) { // the first head's rows with the slot, not behind it: one latency less
         x = *reinterpret_cast<const uint4 *>(ks + h0 * a.k_head_stride);
         y = *reinterpret_cast<const uint4 *>(vs + h0 * a.v_head_stride);
+        slot = a.slots[token];
     }
+    const bool kept = slot >= 0 && slot < a.c.capacity;
+    const int page = kept ? (int)(slot / a.c.page_size) : 0, place = kept ? (int)(slot - (int64_t)page * a.c.page_size) : 0;
+    if (!__any_sync(0xffffffffu, kept))
+        return;
     uint8_t *granule = kv_granule(a.c, page, place, h0, kGranule);
     const size_t head_step = (size_t)(a.c.page_size >> 4) * kGranule;
     for (int h = h0; h < h1; ++h, granule += head_step) {
