@@ -20,6 +20,7 @@
 namespace abq {
 
 constexpr int kKvThreads = 256;
+constexpr int kKvMostRows = 0x7fffff00; // a CTA's last row has a 32-bit number
 
 struct KvShape {
     uint8_t *data;
@@ -253,17 +254,32 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvReadArgs a)
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int sub = threadIdx.x % kLanes, row = blockIdx.x * kTokens + threadIdx.x / kLanes;
-    if (row >= a.rows || row >= a.cu_seqlens[a.batch])
-        return;
-    int lo = 0, hi = a.batch; // the sequence with cu[lo] <= row < cu[lo + 1]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu_seqlens[mid] <= row)
-            lo = mid;
-        else
-            hi = mid;
+    int lo = 0, start, end; // the sequence with cu[lo] <= row < cu[lo + 1]
+    if (a.batch < 32) {     // one load, a place a lane
+        const int lane = threadIdx.x & 31, mine = a.cu_seqlens[min(lane, a.batch)], first = row - lane / kLanes;
+#pragma unroll
+        for (int j = 0; j < 32 / kLanes; ++j) {
+            const uint32_t before = __ballot_sync(0xffffffffu, lane < a.batch && mine <= first + j);
+            if (lane / kLanes == j)
+                lo = max(0, 31 - __clz((int)before));
+        }
+        start = __shfl_sync(0xffffffffu, mine, lo);
+        end = __shfl_sync(0xffffffffu, mine, a.batch);
+    } else {
+        int hi = a.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.cu_seqlens[mid] <= row)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        start = a.cu_seqlens[lo];
+        end = a.cu_seqlens[a.batch];
     }
-    const int pos = row - a.cu_seqlens[lo], entry = pos / a.c.page_size, place = pos - entry * a.c.page_size;
+    if (row >= a.rows || row >= end)
+        return;
+    const int pos = row - start, entry = pos / a.c.page_size, place = pos - entry * a.c.page_size;
     const int page = entry >= 0 && entry < a.table_stride ? a.block_table[(size_t)lo * a.table_stride + entry] : -1;
     const bool held = page >= 0 && page < a.c.num_pages;
     const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(a.c.kv_heads, h0 + a.heads_per_cta), t = place & 15;
@@ -366,7 +382,7 @@ extern "C" size_t abq_kv_cache_bytes(const abq_kv_cache *cache)
 extern "C" abq_status abq_kv_cache_write(const abq_kv_write_params *p, abq_stream_t stream)
 {
     using namespace abq;
-    if (!p || !kv_cache_valid(p->cache) || !p->cache.data || (reinterpret_cast<uintptr_t>(p->cache.data) & 15) || p->tokens < 0)
+    if (!p || !kv_cache_valid(p->cache) || !p->cache.data || (reinterpret_cast<uintptr_t>(p->cache.data) & 15) || p->tokens < 0 || p->tokens > kKvMostRows)
         return ABQ_ERR_INVALID_ARG;
     if (p->tokens == 0)
         return ABQ_OK;
@@ -385,7 +401,7 @@ extern "C" abq_status abq_kv_cache_write(const abq_kv_write_params *p, abq_strea
 extern "C" abq_status abq_kv_cache_read(const abq_kv_read_params *p, abq_stream_t stream)
 {
     using namespace abq;
-    if (!p || !kv_cache_valid(p->cache) || !p->cache.data || (reinterpret_cast<uintptr_t>(p->cache.data) & 15) || p->rows < 0 || p->batch < 0)
+    if (!p || !kv_cache_valid(p->cache) || !p->cache.data || (reinterpret_cast<uintptr_t>(p->cache.data) & 15) || p->rows < 0 || p->rows > kKvMostRows || p->batch < 0)
         return ABQ_ERR_INVALID_ARG;
     if (p->rows == 0 || p->batch == 0)
         return ABQ_OK;

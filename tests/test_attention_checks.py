@@ -50,7 +50,7 @@ ROW_FAULTS = [dict(k=None), dict(v=4098), dict(k_stride=260), dict(v_head_stride
 def test_write_refuses(abq):
     good = dict(cache=_cache(abq), k=4096, v=4096, k_stride=256, k_head_stride=128, v_stride=256, v_head_stride=128, slots=4096, tokens=3)
     _refused(abq.lib().abq_kv_cache_write, abq.KVWriteParams, good,
-             ROW_FAULTS + [dict(slots=None), dict(slots=4100), dict(tokens=-1)] + [dict(cache=_cache(abq, **c)) for c in CACHE_FAULTS])
+             ROW_FAULTS + [dict(slots=None), dict(slots=4100), dict(tokens=-1), dict(tokens=2**31 - 1)] + [dict(cache=_cache(abq, **c)) for c in CACHE_FAULTS])
     p = abq.KVWriteParams()
     for k, v in {**good, "tokens": 0, "k": None, "v": None, "slots": None}.items():
         setattr(p, k, v)
@@ -61,7 +61,7 @@ def test_read_refuses(abq):
     good = dict(cache=_cache(abq), k=4096, v=4096, k_stride=256, k_head_stride=128, v_stride=256, v_head_stride=128, rows=3, batch=1, block_table=4096, table_stride=4,
                 cu_seqlens=4096)
     _refused(abq.lib().abq_kv_cache_read, abq.KVReadParams, good,
-             ROW_FAULTS + [dict(block_table=None), dict(block_table=4098), dict(cu_seqlens=None), dict(table_stride=0), dict(rows=-1), dict(batch=-1)] +
+             ROW_FAULTS + [dict(block_table=None), dict(block_table=4098), dict(cu_seqlens=None), dict(table_stride=0), dict(rows=-1), dict(rows=2**31 - 1), dict(batch=-1)] +
              [dict(cache=_cache(abq, **c)) for c in CACHE_FAULTS])
 
 

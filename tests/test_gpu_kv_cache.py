@@ -113,3 +113,27 @@ def test_pages_outside_the_cache_read_as_zero(abq, cuda):
     abq.kv_cache_read(abq.make_kv_read_params(cache, k, v, table, torch.tensor([0, 80], dtype=torch.int32).cuda()))
     zero = (k == 0).all(-1).view(5, 16).all(1).cpu()
     assert zero.tolist() == [False, True, True, False, True]
+
+
+@pytest.mark.parametrize("batch", [31, 32, 70])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_sequences_read_together_as_one_by_one(abq, cuda, batch, dim):
+    """Empty ones among them, at the start, in a row, and at the end."""
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(1, 40, (batch,), generator=gen)
+    lens[[0, 1, 5, 6, 7, batch - 1]] = 0
+    table = torch.randperm(3 * batch, generator=gen).to(torch.int32).view(batch, 3).cuda()
+    held = torch.zeros(abq.kv_cache_bytes(3 * batch, 16, 2, dim, 8), dtype=torch.uint8, device="cuda")
+    cache = abq.make_kv_cache(held, page_size=16, kv_heads=2, head_dim=dim, bits=8, dtype=torch.float16)
+    k, v = _rows(gen, 48 * batch, 2, dim, torch.float16)
+    abq.kv_cache_write(abq.make_kv_write_params(cache, k, v, torch.arange(48 * batch).cuda()))
+    cu = [0] + lens.cumsum(0).tolist()
+    rows = torch.full((2, cu[-1] + 9, 2, dim), -9.0, dtype=torch.float16, device="cuda")
+    abq.kv_cache_read(abq.make_kv_read_params(cache, rows[0], rows[1], table, torch.tensor(cu, dtype=torch.int32).cuda()))
+    for b in range(batch):
+        n = cu[b + 1] - cu[b]
+        if n:
+            one = torch.empty((2, n, 2, dim), dtype=torch.float16, device="cuda")
+            abq.kv_cache_read(abq.make_kv_read_params(cache, one[0], one[1], table[b:b + 1], torch.tensor([0, n], dtype=torch.int32).cuda()))
+            assert torch.equal(one, rows[:, cu[b]:cu[b + 1]]), b
+    assert bool((rows[:, cu[-1]:] == -9).all())
