@@ -10,7 +10,7 @@
 // close to the middle between two codes), or whose scale is below the normal range, is divided.  The scale is rounded up to 16 bits, so max never passes the
 // last code.
 //
-// Measured: 16001 tokens of 32 heads of 128, fp16 and 4 bits (332 MB either way): written in 83 us (4.0 TB/s; bound by instructions: 135 before the arithmetic was
+// Measured: 16001 tokens of 32 heads of 128, fp16 and 4 bits (332 MB either way): written in 81 us (4.1 TB/s; bound by instructions: 135 before the arithmetic was
 // packed and the divisions taken out, 90 with every lane working out both rows' parameters), read back in 55 us (6.0 TB/s, 92 % of a copy's rate).
 #include <type_traits>
 
