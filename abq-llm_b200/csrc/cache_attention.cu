@@ -28,7 +28,7 @@ static CaPlan ca_plan(int rows, int head_dim)
     if (rows >= 80 * blocks) // (measured: see there)
         return { true, 128, kCaSms, 7, 2, 2 }; // (an item counts for two tiles more; with 1, 2, 3: 31.0, 29.8, 31.1 us for 16 trees of 64 rows, 41.7, 38.5, 41.2 for four)
     const int tiles = row_tiles(rows);
-    return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(head_dim, tiles) * kCaWarps, 4, kCaExtra, kCaMinQuota };
+    return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(head_dim, tiles) * kCaWarps, 4, kCaExtra, ca_min_quota(tiles) };
 }
 
 static bool attention_shape_valid(const abq_kv_cache &c, int batch, int n, int q_heads)

@@ -14,7 +14,7 @@
 // too few loads under way.
 //
 // Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 95 (76.7, so 81 % of the rate); 32 of
-// up to 4096 tokens, 4 bits 20.2 (4.8); one of 1024 tokens, 32 heads 8.9 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for
+// up to 4096 tokens, 4 bits 20.0 (4.8); one of 1024 tokens, 32 heads 8.0 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for
 // the second kernel, are what short calls cost.
 //
 //  * Running maximum: raised only when a score passes it by more than 2^8 (checked with one vote), so that shuffles and the scaling of O are rare.
@@ -35,7 +35,9 @@ namespace abq {
 constexpr int kCaWarps = 4;
 constexpr int kCaThreads = 32 * kCaWarps;
 constexpr int kCaSms = 148;
-constexpr int kCaMinQuota = 4; // granules a warp takes at least
+// Granules a warp takes at least: fewer take less time, but more pieces have to be joined.  Measured with 1, 2, 3, 4, 6 (us, 32 heads): one sequence of 1024 tokens, one row 9.1 8.0
+// 8.6 8.8 10.1; of 300 6.9 7.1 7.8 8.6 10.0; 12 rows on 8 key heads, 1024 tokens 12.7 12.7 11.3 11.6 12.9.
+__host__ __device__ constexpr int ca_min_quota(int tiles) { return tiles == 1 ? 2 : 3; }
 // What an item costs beside its granules, in granules.  Measured with 1, 2, 3, 4, 5, 6 (us): 29 sequences of up to 4096 tokens, one row 21.5 20.7 20.0 20.2 19.9 19.9; 4 of up to
 // 2049, 26 rows 35.4 35.6 34.4 33.7 33.7 35.0; one of 1024, one row 9.9 8.9 9.1 9.0 8.9 9.0.
 constexpr int kCaExtra = 4;
