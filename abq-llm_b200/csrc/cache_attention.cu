@@ -26,7 +26,7 @@ static CaPlan ca_plan(int rows, int head_dim)
 {
     const int blocks = (rows + 127) / 128;
     if (rows >= 80 * blocks) // (measured: see there)
-        return { true, 128, kCaSms, 7, 2, 2 }; // (an item counts for two tiles more; with 1, 2, 3: 31.0, 29.8, 31.1 us for 16 trees of 64 rows, 41.7, 38.5, 41.2 for four)
+        return { true, 128, kCaSms, 7, 2, 1 }; // (an item counts for two tiles more; with 1, 2, 3: 31.0, 29.8, 31.1 us for 16 trees of 64 rows, 41.7, 38.5, 41.2 for four; at least one tile a CTA: with two 18.3 instead of 16.7 for 1000 tokens)
     const int tiles = row_tiles(rows);
     return { false, 8 * tiles, kCaSms * ca_ctas_per_sm(head_dim, tiles) * kCaWarps, 4, kCaExtra, ca_min_quota(tiles) };
 }
