@@ -277,10 +277,11 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvReadArgs a)
         start = a.cu_seqlens[lo];
         end = a.cu_seqlens[a.batch];
     }
-    if (row >= a.rows || row >= end)
+    start = max(start, 0);
+    if (row >= a.rows || row >= end || row < start) // (rows before the first sequence have no position: a negative one would lie in front of its page)
         return;
     const int pos = row - start, entry = pos / a.c.page_size, place = pos - entry * a.c.page_size;
-    const int page = entry >= 0 && entry < a.table_stride ? a.block_table[(size_t)lo * a.table_stride + entry] : -1;
+    const int page = entry < a.table_stride ? a.block_table[(size_t)lo * a.table_stride + entry] : -1;
     const bool held = page >= 0 && page < a.c.num_pages;
     const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(a.c.kv_heads, h0 + a.heads_per_cta), t = place & 15;
     const int at = kv_place<RB>(t, sub * BITS);

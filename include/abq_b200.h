@@ -396,7 +396,8 @@ ABQ_API abq_status abq_kv_cache_write(const abq_kv_write_params *params, abq_str
 
 /*
  * Read whole sequences back, packed: row cu_seqlens[b] + t of k and v gets position t of sequence b.  Feeds abq_prompt_attention with the
- * prefix of a chunk.  Rows from cu_seqlens[batch] on are left as they were; positions whose page is outside the table's row or the cache give 0.
+ * prefix of a chunk.  Rows before cu_seqlens[0] and from cu_seqlens[batch] on are left as they were; positions whose page is outside the table's row or the
+ * cache give 0.
  */
 typedef struct abq_kv_read_params {
     abq_kv_cache cache;
