@@ -261,8 +261,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + kStages * kTile);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *s_read = bars + 8, *o_done = bars + 10, *drain = bars + 12, *half_way = bars + 13;
     uint64_t *kv_full = bars + 15, *kv_empty = kv_full + kStages, *edge_full = kv_empty + kStages;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(edge_full + kStages);
-    int *poison = reinterpret_cast<int *>(tmem_slot + 2); // [2 warps][4 blocks]: V tiles of the block held Inf or NaN
+    uint64_t *flag_read = edge_full + kStages; // [2 row tiles][4]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(flag_read + 8);
+    // [2 row tiles][4][2 warps]: the V tiles that this row tile's rows do not all see to the end held Inf or NaN.  Slots go round over the blocks in which the row tile
+    // has such V tiles: only these are written for it and read by it, and a slot is written again when its four warps have read it (flag_read).
+    int *poison = reinterpret_cast<int *>(tmem_slot + 2);
 
     // No barrier completes a phase before everybody who waits for the one before has seen that: a parity that is asked for two phases late looks like one
     // that has not come.  s_full: the scores of the next keys follow p_ready (or s_read), which follows the wait for these.  o_done: the next product it
@@ -278,6 +281,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             mbar_init(&s_read[t], 4);
             mbar_init(&o_done[t], 1);
             mbar_init(&half_way[t], 4);
+            for (int i = 0; i < 4; ++i)
+                mbar_init(&flag_read[4 * t + i], 4);
         }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&kv_full[s], 2); // the producer twice, or the two warps that looked through the tile
@@ -314,7 +319,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
         const uint32_t ts = tmem + lanes + (uint32_t)(t * 128), tp = tmem + lanes + (uint32_t)(Sh::kP + t * Sh::kPStep), to = tmem + lanes + (uint32_t)(Sh::kO + t * D);
         const int pack = 1 << a.pack_log2;
         uint32_t phase = 0, done = 0, others = 0; // of s_full; of o_done (a product with V each, or with S and P in one place a block); key tiles of the other row tile so far
-        int blocks = 0;               // with a key
+        uint32_t flags = 0;           // flags read
         bool ok = true;
         PaItem next = pa_item(a, number(0), lane);
         for (int round = 0; ok; ++round) {
@@ -456,10 +461,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 pa_unpack(sum2, lo, hi);
                 l += lo + hi;
                 inv = l == 0.f ? 0.f : 1.f / l;
-                if (it.edge < n) // (its tiles have been looked through by now; the other tile's may not)
-                    foul = *reinterpret_cast<volatile int *>(&poison[blocks & 3]) | *reinterpret_cast<volatile int *>(&poison[4 + (blocks & 3)]);
+                if (it.edge < n) { // (its V tiles have been looked through by now; the other row tile's may not)
+                    const int slot = 4 * t + (flags & 3);
+                    foul = *reinterpret_cast<volatile int *>(&poison[2 * slot]) | *reinterpret_cast<volatile int *>(&poison[2 * slot + 1]);
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(&flag_read[slot]);
+                    ++flags;
+                }
             }
-            blocks += it.most > 0;
             others += t ? it.n[0] : it.n[1];
             // Four lanes exchange their 16-byte pieces, so that a store covers 64 bytes of 8 rows and not 16 of 32: lane 4 a + b gets piece b of rows 4 a ..
             uint8_t *dst[4];
@@ -695,8 +705,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     } else {
         // ---------------------------------------------------------------- V tiles that are not seen to the end
         const int half = warp - 10;
-        int place = 0, blocks = 0;
-        uint32_t edges = 0;
+        int place = 0;
+        uint32_t edges = 0, flags[2] = { 0, 0 }; // flags written, per row tile
         bool ok = true;
         for (int round = 0; ok; ++round) {
             const PaItem it = pa_item(a, number(round), lane);
@@ -704,6 +714,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 break;
             if (it.most == 0)
                 continue;
+            // A flag's phase cannot be two ahead of this wait: its next reader needs the flag that is written behind it
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (it.edge < it.n[t] && flags[t] >= 4)
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&flag_read[4 * t + (flags[t] & 3)], ((flags[t] >> 2) - 1) & 1, a.status, STATUS_TIMEOUT_PIPE));
+            if (!ok)
+                break;
             int bad = 0;
             for (int j = it.edge; j < it.most; ++j) {
                 const int s = (place + pa_v_place(j, it.most)) % kStages;
@@ -736,15 +753,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                     }
                 }
                 bad = __any_sync(0xffffffffu, bad);
-                if (lane == 0)
-                    poison[4 * half + (blocks & 3)] = bad; // (copies run at most two blocks ahead of the softmax)
+                if (lane == 0) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (j < it.n[t])
+                            poison[2 * (4 * t + (flags[t] & 3)) + half] = bad;
+                }
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&kv_full[s]);
             }
             place += 2 * it.most;
-            ++blocks;
+            flags[0] += it.edge < it.n[0];
+            flags[1] += it.edge < it.n[1];
         }
     }
 
