@@ -13,7 +13,7 @@ tree of drafted tokens, whole prompts, or a chunk of a prompt behind what the ca
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, List, Sequence
 
 from . import binding as B
@@ -100,6 +100,7 @@ class AttentionStep:
     cu_k: object
     tree: object = None
     workspace: object = None
+    outgrown: list = field(default_factory=list)  # workspaces that were too small for a later layer: a captured launch may still point to them
 
     @classmethod
     def make(cls, torch, sequences: PagedSequences, ids: Sequence[int], new: Sequence[int], *, prompt: bool, tree=None, device="cuda") -> "AttentionStep":
@@ -124,10 +125,19 @@ class AttentionStep:
                    block_table=ints([p + [0] * (width - len(p)) for p in pages], torch.int32), seq_lens=ints(lens, torch.int32),
                    cu_q=ends(new), cu_k=ends(lens), tree=tree)
 
+    def scratch(self, torch, nbytes: int, device):
+        """The step's workspace, with room for ``nbytes``.  It lives as long as the step, and so do the smaller ones before it."""
+        if self.workspace is None or self.workspace.numel() < nbytes:
+            if self.workspace is not None:
+                self.outgrown.append(self.workspace)
+            self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return self.workspace
+
 
 class BlockAttention:
     """One layer's quantised cache and its attention.  ``step`` is set by the caller before a forward pass; calls write the step's keys
-    and values into the cache, then attend.  All on the current stream; the layers of a model share a step (and its workspace)."""
+    and values into the cache, then attend.  All on the current stream; the layers of a model share a step (and its workspace, so calls that
+    may overlap need a step each).  A captured launch reads the step's tables and uses its workspace: the caller keeps the step as long as the graph."""
 
     def __init__(self, abq, torch, *, heads: int, kv_heads: int | None = None, head_dim: int = 128, num_pages: int, page_size: int = 16, bits: int = 8, dtype=None,
                  scale: float | None = None, device="cuda", status_word=None):
@@ -163,10 +173,8 @@ class BlockAttention:
         B.kv_cache_write(B.make_kv_write_params(self.cache, k, v, step.slots))
         if step.kind == "tokens":
             need = B.cache_attention_workspace_bytes(self.cache, step.seq_lens.numel(), step.rows, self.heads)
-            if step.workspace is None or step.workspace.numel() < need:
-                step.workspace = torch.empty(need, dtype=torch.uint8, device=qkv.device)
-            B.cache_attention(B.make_cache_attention_params(self.cache, q, res, step.block_table, step.seq_lens, scale=self.scale, workspace=step.workspace, tree=step.tree,
-                                                            status_word=self.status_word))
+            B.cache_attention(B.make_cache_attention_params(self.cache, q, res, step.block_table, step.seq_lens, scale=self.scale,
+                                                            workspace=step.scratch(torch, need, qkv.device), tree=step.tree, status_word=self.status_word))
             return out
         if step.prefix:  # a chunk behind what the cache holds: whole sequences come out of it, the chunk as it has just been written among them
             k, v = (torch.empty((step.held, self.kv_heads, self.head_dim), dtype=self.dtype, device=qkv.device) for _ in range(2))
