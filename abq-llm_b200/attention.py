@@ -41,7 +41,7 @@ class PagedSequences:
         self._pages[seq], self._length[seq] = [], 0
         try:
             self.extend(seq, tokens)
-        except OutOfPages:
+        except (OutOfPages, ValueError):
             del self._pages[seq], self._length[seq]
             raise
         self._next += 1
@@ -79,7 +79,7 @@ class PagedSequences:
     def slots(self, seq: int, tokens: int) -> List[int]:
         """Places of the last ``tokens`` tokens, as abq_kv_cache_write takes them."""
         n, P = self._length[seq], self.page_size
-        if tokens > n:
+        if not 0 <= tokens <= n:
             raise ValueError(f"sequence {seq} has {n} tokens")
         return [self._pages[seq][t // P] * P + t % P for t in range(n - tokens, n)]
 
