@@ -44,11 +44,15 @@ class LinearSpec:
     out_features: int
     in_features: int
     parallel: str  # "column" (split out_features) or "row" (split in_features, all-reduce after)
+    heads_per_kv: int = 1  # "qkv" and "o": query heads that share a key head
 
 
-def llama_block_specs(hidden: int, ffn: int) -> List[LinearSpec]:
-    """The four quantized GEMMs of a block as FasterTransformer runs them: fused QKV, O, fused gate+up, down."""
-    return [LinearSpec("qkv", 3 * hidden, hidden, "column"), LinearSpec("o", hidden, hidden, "row"),
+def llama_block_specs(hidden: int, ffn: int, heads_per_kv: int = 1) -> List[LinearSpec]:
+    """The four quantized GEMMs of a block as FasterTransformer runs them: fused QKV, O, fused gate+up, down.  With grouped heads the QKV projection has
+    hidden + 2 * hidden / heads_per_kv outputs: queries, keys, values."""
+    if heads_per_kv < 1 or hidden % heads_per_kv:
+        raise ValueError(f"{hidden} query features, {heads_per_kv} query heads a key head")
+    return [LinearSpec("qkv", hidden + 2 * (hidden // heads_per_kv), hidden, "column", heads_per_kv), LinearSpec("o", hidden, hidden, "row", heads_per_kv),
             LinearSpec("gate_up", 2 * ffn, hidden, "column"), LinearSpec("down", hidden, ffn, "row")]
 
 
@@ -56,12 +60,13 @@ def shard_of(spec: LinearSpec, rank: int, world: int, unit: int = 128) -> Tuple[
     """(rows, columns) of the full [out_features][in_features] code matrix that ``rank`` owns."""
     if spec.parallel == "column":
         # fused layers (qkv, gate_up) are split per fused part so that every rank holds matching slices of each
-        parts = 3 if spec.name == "qkv" else (2 if spec.name == "gate_up" else 1)
-        per = spec.out_features // parts
-        b, e = unit_ranges(per, world, unit)[rank]  # the same ranges as the K split of the row-parallel layer that follows
-        rows = [i for p in range(parts) for i in range(p * per + b, p * per + e)]
+        g = spec.heads_per_kv
+        parts = [g, 1, 1] if spec.name == "qkv" else ([1, 1] if spec.name == "gate_up" else [1])
+        per = spec.out_features // sum(parts)
+        b, e = unit_ranges(per, world, unit)[rank]  # the same ranges as the K split of the row-parallel layer that follows; g times as wide for queries
+        rows = [i for p, width in enumerate(parts) for i in range(sum(parts[:p]) * per + width * b, sum(parts[:p]) * per + width * e)]
         return rows, slice(0, spec.in_features)
-    b, e = unit_ranges(spec.in_features, world, unit)[rank]
+    b, e = unit_ranges(spec.in_features, world, unit * spec.heads_per_kv)[rank]
     return slice(0, spec.out_features), slice(b, e)
 
 
@@ -71,15 +76,33 @@ class TensorParallelBlockLinears:
     ``backend.make_linear(codes, scale, zero, w_bits, group, reduce_output=...)`` returns an object with
     ``__call__(x_half) -> fp16``; ``backend.all_reduce(t)`` returns the sum over ranks (in ``t`` or in a tensor of its own); ``backend.glue`` supplies the elementwise stand-ins between the
     GEMMs.  ``attention(qkv, out)``, if given (attention.BlockAttention: this rank's heads over a quantised cache), runs between the QKV and
-    the output projection; without it the first third of the QKV output stands in for its result.
+    the output projection; without it the queries in the QKV output stand in for its result.  It may be any callable (one that turns queries
+    and keys by their positions first, say).
+
+    ``heads_per_kv``: query heads that share a key head; None takes it from ``attention`` where that says its heads.  Key heads are dealt
+    to the ranks in whole units of 128 features, each with its query heads.
     """
 
-    def __init__(self, backend, hidden: int, ffn: int, rank: int, world: int, weights: Sequence, w_bits: int, group: int = 0, attention=None):
+    def __init__(self, backend, hidden: int, ffn: int, rank: int, world: int, weights: Sequence, w_bits: int, group: int = 0, attention=None, heads_per_kv: int | None = None):
         self.backend, self.hidden, self.ffn, self.rank, self.world = backend, hidden, ffn, rank, world
         self.attention = attention
-        self.specs = llama_block_specs(hidden, ffn)
+        of = {n: getattr(attention, n, None) for n in ("heads", "kv_heads", "head_dim", "dtype")}
+        if heads_per_kv is None:
+            heads_per_kv = of["heads"] // of["kv_heads"] if of["heads"] and of["kv_heads"] else 1
+        self.heads_per_kv = heads_per_kv
+        self.specs = llama_block_specs(hidden, ffn, heads_per_kv)
+        if of["heads"] and of["kv_heads"] and of["head_dim"]:
+            width, own = [(of["heads"] + 2 * of["kv_heads"]) * of["head_dim"], of["heads"] * of["head_dim"]], shard_of(self.specs[1], rank, world)[1]
+            local = [len(shard_of(self.specs[0], rank, world)[0]), own.stop - own.start]
+            if width != local:
+                raise ValueError(f"an attention of {of['heads']} heads on {of['kv_heads']} of {of['head_dim']} reads {width[0]} features and gives {width[1]}; "
+                                 f"rank {rank} of {world} of a block of {hidden}, {heads_per_kv} heads a key head, has {local[0]} and {local[1]}")
+        if of["dtype"] is not None and str(of["dtype"]) != "torch.float16":
+            raise ValueError(f"the linear layers of a block are fp16, its attention {of['dtype']}")
         self.layers = {}
         for spec, (codes, scale, zero) in zip(self.specs, weights):
+            if tuple(codes.shape) != (spec.out_features, spec.in_features):
+                raise ValueError(f"{spec.name}: codes {tuple(codes.shape)}, expected {(spec.out_features, spec.in_features)}")
             rows, cols = shard_of(spec, rank, world)
             c = codes[rows][:, cols]
             if group:  # per-group parameters follow their K groups
@@ -96,14 +119,15 @@ class TensorParallelBlockLinears:
     def _attention(self, qkv, M):
         if self.attention is not None:
             return self.attention(qkv, self._buf("o", M))
-        return self.backend.glue_attention(qkv, self.layers["qkv"].out_features // 3, self._buf("o", M))
+        g = self.heads_per_kv
+        return self.backend.glue_attention(qkv, self.layers["qkv"].out_features * g // (g + 2), self._buf("o", M))
 
     # The block in the three pieces that lie between its two all-reduces (a caller that replays CUDA graphs captures
     # the pieces and launches the collectives between them):
     def attention_part(self, x):
         """x -> this rank's partial of the attention output projection (to be all-reduced)."""
         be, M = self.backend, x.shape[0]
-        qkv = self.layers["qkv"](x)                                                        # [M][3 * hidden / world]
+        qkv = self.layers["qkv"](x)                                                        # [M][this rank's queries, keys, values]
         attn = self._attention(qkv, M)                                                     # this rank's heads
         return self.layers["o"](attn)                                                      # partial [M][hidden]
 
