@@ -92,7 +92,7 @@ class AttentionStep:
     total: int               # rows of the step
     longest: int             # rows of the sequence with most
     held: int                # tokens of all sequences, those of the step included
-    prefix: bool             # some sequence had tokens before the step
+    prefix: bool             # some sequence had tokens before the step (or read_back): a prompt step's keys and values come out of the cache, for all its sequences
     slots: object
     block_table: object
     seq_lens: object
@@ -103,9 +103,14 @@ class AttentionStep:
     outgrown: list = field(default_factory=list)  # workspaces that were too small for a later layer: a captured launch may still point to them
 
     @classmethod
-    def make(cls, torch, sequences: PagedSequences, ids: Sequence[int], new: Sequence[int], *, prompt: bool, tree=None, device="cuda") -> "AttentionStep":
+    def make(cls, torch, sequences: PagedSequences, ids: Sequence[int], new: Sequence[int], *, prompt: bool, tree=None, read_back: bool = False,
+             device="cuda") -> "AttentionStep":
         """``new`` tokens of every sequence of ``ids`` have places already (:meth:`PagedSequences.extend`).  ``tree``: int64 [batch][rows] as
-        abq_cache_attention takes it."""
+        abq_cache_attention takes it.
+
+        A prompt step in which no sequence had tokens before attends to the keys and values as they come; as soon as one had, all of its sequences attend to what
+        the cache gives back, quantised.  ``read_back``: the latter always, so that a prompt's result depends neither on what it is batched with nor on the chunks
+        that it comes in (it costs reading the step's tokens back)."""
         if len(ids) != len(new) or not ids or any(m < 0 or m > sequences.length(s) for s, m in zip(ids, new)):
             raise ValueError("a step needs a number of new tokens for each of its sequences, at most its length")
         if len(set(ids)) != len(ids):
@@ -120,7 +125,7 @@ class AttentionStep:
         ints = lambda v, t: torch.tensor(v, dtype=t).to(device)  # noqa: E731
         ends = lambda v: ints([sum(v[:i]) for i in range(len(v) + 1)], torch.int32)  # noqa: E731
         return cls(kind="prompt" if prompt else "tokens", rows=0 if prompt else new[0], total=sum(new), longest=max(new), held=sum(lens),
-                   prefix=any(m < n for m, n in zip(new, lens)),
+                   prefix=any(m < n for m, n in zip(new, lens)) or (prompt and read_back),
                    slots=ints([x for s, m in zip(ids, new) for x in sequences.slots(s, m)], torch.int64),
                    block_table=ints([p + [0] * (width - len(p)) for p in pages], torch.int32), seq_lens=ints(lens, torch.int32),
                    cu_q=ends(new), cu_k=ends(lens), tree=tree)
