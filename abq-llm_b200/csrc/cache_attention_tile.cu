@@ -19,7 +19,8 @@
 // and 24.4, 27.0 and 23.6.  So it is taken where its blocks are at least five eighths full.
 //
 // The maximum is looked for at a run's first tile and where the sum over a tile says that it has risen by more than 2^8; the value scales' power of two as in
-// cache_attention.cuh, but as a part of the exponent: p is 2^(s - m) 2^(6 - L) throughout (L at least -60, so that no sum of p overflows).
+// cache_attention.cuh, on the scale that p is multiplied with.  (As a part of p's exponent it saved a multiplication a score, but lost bf16 values below 2^-80 and
+// overflowed in sums of value offsets above 2^50.)
 #include <type_traits>
 
 #include "attention_tmem.cuh"
@@ -180,8 +181,8 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             load_queries(p);
         while (more && ok) {
             const bool live = at < rows, some = __any_sync(0xffffffffu, live); // (of a warp of rows that do not exist nothing is read)
-            float m = live ? -INFINITY : 0.f, mm = 0.f, l = 0.f, bias = 0.f;   // mm = m + L - 6 (no row: nothing to look for)
-            float vmax = 0.f;                                                  // 2^(L + 1)
+            float m = live ? -INFINITY : 0.f, mm = 0.f, l = 0.f, bias = 0.f;   // mm: m, or 0 before the first score (no row: nothing to look for)
+            float vmax = 0.f, vnorm = 1.f;                                     // 2^(L + 1), 2^(6 - L)
             int L = -121;
             const int tiles = p.g1 - p.g0;
             for (int j = 0; j < tiles; ++j, ++T) {
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                                     const float pe = see ? pa_ex2(fmaf(s[4 * g + e], q4.x * rf, fmaf(q4.y, rs, -mm))) : 0.f;
                                     tl += pe;
                                     tb = fmaf(pe, see ? q4.w : 0.f, tb);
-                                    pv[e] = pe * (see ? q4.z : 0.f);
+                                    pv[e] = pe * (see ? q4.z * vnorm : 0.f);
                                 }
                                 w[2 * g] = float_pair_to_half(pv[0], pv[1], false);
                                 w[2 * g + 1] = float_pair_to_half(pv[2], pv[3], false);
@@ -272,16 +273,21 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                             if (!(top < INFINITY)) // NaN (or an overflow): the row's result
                                 l = NAN;
                             const float before = mm;
+                            float down = 1.f;
                             const bool first = m == -INFINITY; // (before the first score of a row its sums are 0, whatever they are multiplied by)
                             if (top > m + 8.f)
                                 m = top;
                             if (vtop >= vmax) {
-                                L = max(L, max((int)(__float_as_uint(vtop) >> 23) - 127, -60));
+                                const int Ln = max(L, max((int)(__float_as_uint(vtop) >> 23) - 127, -120));
+                                down = pa_ex2((float)(L - Ln));
+                                L = Ln;
                                 vmax = __int_as_float(min(128 + L, 255) << 23);
+                                vnorm = __int_as_float((133 - L) << 23);
                             }
-                            mm = m == -INFINITY ? 0.f : m + (float)(L - 6);
+                            mm = m == -INFINITY ? 0.f : m;
                             const float f = first ? 1.f : pa_ex2(before - mm);
-                            if (__any_sync(0xffffffffu, f != 1.f)) {
+                            down *= f; // of O
+                            if (__any_sync(0xffffffffu, down != 1.f)) {
                                 l *= f;
                                 bias *= f;
                                 if (j > 0) {
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                                         uint32_t w[32];
 #pragma unroll
                                         for (int e = 0; e < 32; ++e)
-                                            w[e] = __float_as_uint(o[e] * f);
+                                            w[e] = __float_as_uint(o[e] * down);
                                         pa_st16(to + x, w);
                                         pa_st16(to + x + 16, w + 16);
                                     }
@@ -304,10 +310,10 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
                             weights(std::true_type());
                         else
                             weights(std::false_type());
-                        // no p above 2^8 (in units of 2^(6 - L)), so none times a value scale above 2^15
+                        // no p above 2^8, so none times a value scale above 2^15
                         if (look)
                             break;
-                        look = !__all_sync(0xffffffffu, tl <= __int_as_float((127 + 14 - L) << 23));
+                        look = !__all_sync(0xffffffffu, tl <= 256.f);
                         float2 other;
                         meet(make_float2(look ? 1.f : 0.f, 0.f), other);
                         look = look || other.x != 0.f;
@@ -365,23 +371,21 @@ __global__ void __launch_bounds__(kCtThreads, 1) cache_attention_tile_kernel(con
             };
             float2 *ml = reinterpret_cast<float2 *>(a.part + 2 * (size_t)a.runs * a.slot_rows * D) + slot * a.slot_rows;
             const int to_row = row0 + row;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = l == 0.f ? 0.f : 1.f / l, undo = __int_as_float((121 + L) << 23); // 2^(L - 6); L >= -121
 #pragma unroll 1
             for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 16) {
                 float o[16];
                 pa_ld16(to + x, o);
                 if (to_row < rows) {
-                    if (l == 0.f) { // (P was 0 throughout, or nothing was written to these columns)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            o[e] = 0.f;
-                    }
+                    for (int e = 0; e < 16; ++e)
+                        o[e] = l == 0.f ? 0.f : o[e] * undo; // (0: P was 0 throughout, or nothing was written to these columns)
                     put(to_row, x, o, inv);
                     put(to_row, x + 8, o + 8, inv);
                 }
             }
             if (half == 0 && !whole && to_row < rows)
-                ml[row] = make_float2(l == 0.f ? -INFINITY : mm, l);
+                ml[row] = make_float2(l == 0.f ? -INFINITY : m, l);
             tmem_fence_before(); // (O is read before the next piece's first product, which waits for this warp's p)
         }
     } else if (warp < 16) {
