@@ -261,10 +261,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
     uint64_t *bars = reinterpret_cast<uint64_t *>(ring + kStages * kTile);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *s_read = bars + 8, *o_done = bars + 10, *drain = bars + 12, *half_way = bars + 13;
     uint64_t *kv_full = bars + 15, *kv_empty = kv_full + kStages, *edge_full = kv_empty + kStages;
-    uint64_t *flag_read = edge_full + kStages; // [2 row tiles][4]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(flag_read + 8);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(edge_full + kStages);
     // [2 row tiles][4][2 warps]: the V tiles that this row tile's rows do not all see to the end held Inf or NaN.  Slots go round over the blocks in which the row tile
-    // has such V tiles: only these are written for it and read by it, and a slot is written again when its four warps have read it (flag_read).
+    // has such V tiles: only these are written for it and read by it.  A slot is read before it is written again, four such blocks later: that block's V comes
+    // behind its Q, whose place is free when the scores of the block one or two before (kQBlocks) are made; by then the row tile's scores of the third of these blocks
+    // have been asked for (D = 64) or its p's of it used, and both wait for its softmax to be in the second or later, past the first one's flag.
     int *poison = reinterpret_cast<int *>(tmem_slot + 2);
 
     // No barrier completes a phase before everybody who waits for the one before has seen that: a parity that is asked for two phases late looks like one
@@ -281,8 +282,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
             mbar_init(&s_read[t], 4);
             mbar_init(&o_done[t], 1);
             mbar_init(&half_way[t], 4);
-            for (int i = 0; i < 4; ++i)
-                mbar_init(&flag_read[4 * t + i], 4);
         }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&kv_full[s], 2); // the producer twice, or the two warps that looked through the tile
@@ -464,9 +463,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 if (it.edge < n) { // (its V tiles have been looked through by now; the other row tile's may not)
                     const int slot = 4 * t + (flags & 3);
                     foul = *reinterpret_cast<volatile int *>(&poison[2 * slot]) | *reinterpret_cast<volatile int *>(&poison[2 * slot + 1]);
-                    __syncwarp();
-                    if (lane == 0)
-                        mbar_arrive(&flag_read[slot]);
                     ++flags;
                 }
             }
@@ -714,13 +710,6 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid
                 break;
             if (it.most == 0)
                 continue;
-            // A flag's phase cannot be two ahead of this wait: its next reader needs the flag that is written behind it
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (it.edge < it.n[t] && flags[t] >= 4)
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&flag_read[4 * t + (flags[t] & 3)], ((flags[t] >> 2) - 1) & 1, a.status, STATUS_TIMEOUT_PIPE));
-            if (!ok)
-                break;
             int bad = 0;
             for (int j = it.edge; j < it.most; ++j) {
                 const int s = (place + pa_v_place(j, it.most)) % kStages;
