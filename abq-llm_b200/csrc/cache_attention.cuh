@@ -13,9 +13,9 @@
 // workspace, added by a second kernel in order (no atomics): joined by whichever warp comes last they took twice the time of both kernels, since one warp has
 // too few loads under way.
 //
-// Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 95 (76.7, so 81 % of the rate); 32 of
-// up to 4096 tokens, 4 bits 20.0 (4.8); one of 1024 tokens, 32 heads 8.0 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for
-// the second kernel, are what short calls cost.
+// Measured (us, one call in a chain; the bytes' floor at the copy rate): 2 sequences of 128 K tokens, 32 heads on 8, 8 bits 95 to 99 (76.7, so 78 to 81 % of the rate); 32 of
+// up to 4096 tokens, 4 bits 20.6 (4.8): a granule is a chain of dependent steps of 1750 clocks for its warp, three warps a scheduler; one of 1024 tokens, 32 heads 8.0
+// to 8.5 (1.3): 3 us until a warp has found its run and its first copy is there, and 3 us for the second kernel, are what short calls cost.
 //
 //  * Running maximum: raised only when a score passes it by more than 2^8 (checked with one vote), so that shuffles and the scaling of O are rare.
 //  * p vs_j is rounded to fp16 after scaling by a power of two that keeps the largest vs seen so far near 2^6: with p <= 2^8 the product is below 2^15 and
@@ -23,8 +23,9 @@
 //    is multiplied too (a second MMA per tile): rounded alone it would be an error as large as the result's own rounding.  With more rows, where the products
 //    count, it is left out; bf16 results do not show it.
 //  * Keys are multiplied as 1024 + c (8 bits) or 1 + c / 64 (4 bits), which are single logic operations away from the codes; the constant times sum(q) goes
-//    with the row's offset.  Over the 8 steps of one score that costs at most 2^-23 of 1024 sum|q|; values are summed over thousands of tokens and are
-//    multiplied centred.
+//    with the row's offset.  The running sum of one score's D / 16 products is rounded at each of them, at a size of up to (1024 + 255) sum|q| (64 + 15 with 4 bits):
+//    at most D / 16 times 2^-23 of that, 2^-20 for D = 128.  In practice it is far less: over 1024 tokens of 8 bits the result's error against 64 bits (2.1e-4,
+//    fp16) is that of its own rounding.  Values are summed over thousands of tokens and are multiplied centred.
 //  * Queries: fp16 as they are; bf16 rows are scaled by a power of two to [1, 2) and held in fp16 (exact down to 2^-14 of the row's largest).
 #pragma once
 #include "abq_kernels.h"

@@ -10,8 +10,9 @@
 // close to the middle between two codes), or whose scale is below the normal range, is divided.  The scale is rounded up to 16 bits, so max never passes the
 // last code.
 //
-// Measured: 16001 tokens of 32 heads of 128, fp16 and 4 bits (332 MB either way): written in 81 us (4.1 TB/s; bound by instructions: 135 before the arithmetic was
-// packed and the divisions taken out, 90 with every lane working out both rows' parameters), read back in 55 us (6.0 TB/s, 92 % of a copy's rate).
+// Measured: 16001 tokens of 32 heads of 128, fp16 and 4 bits (332 MB either way): written in 76 to 81 us (4.1 to 4.4 TB/s; bound by instructions: 135 before the arithmetic was
+// packed and the divisions taken out, 90 with every lane working out both rows' parameters), read back in 62 us (5.4 TB/s, 82 % of a copy's rate), 55 behind the write, part
+// of the cache still in L2; 8 bits (398 MB) written in 78 us (5.1 TB/s), read in 70 (5.7).
 #include <type_traits>
 
 #include "abq_kernels.h"

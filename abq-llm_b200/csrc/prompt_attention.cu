@@ -20,10 +20,10 @@
 // bf16), n added to the exponent.  Tiles with masked scores take the units' function for all (it gives the 0 that they need).  A share of one in eight measured best for
 // heads of 64 (none 137.5 us, one 133.1, two 134.4); more costs more issue slots than the units save.
 //
-// Measured: a prompt of 2048, 32 heads of 128, bf16: 43.7 us (0.79 PFLOP/s, half of the measured bf16 rate); of 8192, 32 heads on 8: 460 us in short bursts (1.20
-// PFLOP/s), 537 sustained, where the power limit lowers the clock; heads of 64, 16 prompts of up to 1023 behind a prefix of 517 each, 32 heads on 4: 113 us (0.45).
-// A pair of tiles over 128 keys takes 3100 clocks for D = 128: softmax 1750 and the products 1100 that it waits for.  Two threads a row (16 softmax warps), the product
-// of P started on half of its columns, and no maximum per tile were no faster.
+// Measured: a prompt of 2048, 32 heads of 128, bf16: 44 to 46 us in a graph (0.75 PFLOP/s), 49 in a loop of calls; of 8192, 32 heads on 8: 460 to 485 us in short bursts (1.15
+// PFLOP/s), 524 to 540 sustained, where the power limit lowers the clock; heads of 64, 16 prompts of up to 1023 behind a prefix of 517 each, 32 heads on 4: 113 to 122 us (0.42).
+// In clocks: a pair of tiles over 128 keys 3100 to 3550 (D = 128: softmax 1750 and the products 1100 that it waits for); a block 2400 to 3900 until its first scores and about
+// 4000 for its result.  Two threads a row (16 softmax warps), the product of P started on half of its columns, and no maximum per tile were no faster.
 //
 // P is rounded to the 16-bit type (tensor-core operands); fp16 holds p times 2^6, so that weights down to 2^-20 of the maximum keep all bits.  The sum of p is
 // that of the unrounded values.

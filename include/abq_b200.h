@@ -416,7 +416,8 @@ ABQ_API abq_status abq_kv_cache_read(const abq_kv_read_params *params, abq_strea
  * (n = 1), or a tree of drafted tokens that are verified at once.  Sequence b holds seq_lens[b] tokens; token seq_lens[b] - n + j is draft j.
  * Row i sees every token before the drafts, and draft j where bit j of tree[b][i] is set (without `tree`: j <= i).  A row that sees no
  * token gives 0 (a sequence of length 0 among them).  out = sum_j softmax_j(scale * q . k_j) v_j in fp32; products run on the tensor cores in
- * fp16, on codes that fp16 holds exactly.
+ * fp16, on codes that fp16 holds exactly.  The sum over j is divided at the end and holds weights of up to 2^8: bf16 values overflow where 2^8 times their magnitude
+ * times the tokens passes 2^128.
  * Lengths are read on the device (a captured launch follows them); they are bounded by table_stride * page_size.  Pages outside the
  * cache are not read: their tokens count as unseen and ABQ_STATUS_BAD_PAGE is set in the status word, if there is one.
  * The workspace is scratch of this call alone: calls that may overlap need one each.
@@ -445,7 +446,7 @@ ABQ_API abq_status abq_cache_attention(const abq_cache_attention_params *params,
  * are its keys and values.  Row i of a sequence of n queries and m keys sees keys 0 .. i + m - n: with m > n the queries are the last of the
  * keys' tokens (a chunk of a prompt behind its prefix), and a row that sees no key (m < n) gives 0.  Rows of `out` from cu_q[batch] on are left as
  * they were.  Keys and values that a row does not see may hold anything, Inf and NaN included.  Products run on the tensor cores in the 16-bit type, sums and
- * the softmax in fp32; p is rounded to the 16-bit type.
+ * the softmax in fp32; p is rounded to the 16-bit type.  (bf16 values overflow where 2^8 times their magnitude times the keys passes 2^128.)
  * Strides of dimensions longer than one are positive.  The call reads nothing back and allocates nothing; it may be captured.
  */
 typedef struct abq_prompt_attention_params {
