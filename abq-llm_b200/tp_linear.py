@@ -86,19 +86,21 @@ class TensorParallelBlockLinears:
     def __init__(self, backend, hidden: int, ffn: int, rank: int, world: int, weights: Sequence, w_bits: int, group: int = 0, attention=None, heads_per_kv: int | None = None):
         self.backend, self.hidden, self.ffn, self.rank, self.world = backend, hidden, ffn, rank, world
         self.attention = attention
-        of = {n: getattr(attention, n, None) for n in ("heads", "kv_heads", "head_dim", "dtype")}
+        shape = [getattr(attention, n, None) for n in ("heads", "kv_heads", "head_dim")]
+        told = all(isinstance(x, int) and x > 0 for x in shape)  # (another callable may have anything by these names)
         if heads_per_kv is None:
-            heads_per_kv = of["heads"] // of["kv_heads"] if of["heads"] and of["kv_heads"] else 1
+            heads_per_kv = shape[0] // shape[1] if told else 1
         self.heads_per_kv = heads_per_kv
         self.specs = llama_block_specs(hidden, ffn, heads_per_kv)
-        if of["heads"] and of["kv_heads"] and of["head_dim"]:
-            width, own = [(of["heads"] + 2 * of["kv_heads"]) * of["head_dim"], of["heads"] * of["head_dim"]], shard_of(self.specs[1], rank, world)[1]
-            local = [len(shard_of(self.specs[0], rank, world)[0]), own.stop - own.start]
-            if width != local:
-                raise ValueError(f"an attention of {of['heads']} heads on {of['kv_heads']} of {of['head_dim']} reads {width[0]} features and gives {width[1]}; "
-                                 f"rank {rank} of {world} of a block of {hidden}, {heads_per_kv} heads a key head, has {local[0]} and {local[1]}")
-        if of["dtype"] is not None and str(of["dtype"]) != "torch.float16":
-            raise ValueError(f"the linear layers of a block are fp16, its attention {of['dtype']}")
+        if told:
+            heads, kv_heads, head_dim = shape
+            own = shard_of(self.specs[1], rank, world)[1]
+            reads, gives = (heads + 2 * kv_heads) * head_dim, heads * head_dim
+            if (reads, gives) != (len(shard_of(self.specs[0], rank, world)[0]), own.stop - own.start):
+                raise ValueError(f"an attention of {heads} heads on {kv_heads} of {head_dim} reads {reads} features and gives {gives}; rank {rank} of {world} of a block of "
+                                 f"{hidden}, {heads_per_kv} heads a key head, has {len(shard_of(self.specs[0], rank, world)[0])} and {own.stop - own.start}")
+            if str(getattr(attention, "dtype", "torch.float16")) != "torch.float16":
+                raise ValueError(f"the linear layers of a block are fp16, its attention {attention.dtype}")
         self.layers = {}
         for spec, (codes, scale, zero) in zip(self.specs, weights):
             if tuple(codes.shape) != (spec.out_features, spec.in_features):

@@ -108,6 +108,19 @@ def test_refusals(tp):
         tp.llama_block_specs(512, 256, 3)
 
 
+def test_other_callables_are_taken_as_they_are(tp):
+    """Names that mean something else there, and a type of its own, are not looked at."""
+    class Own:
+        heads, kv_heads, head_dim, dtype = [1, 2], {}, "64", torch.bfloat16
+
+        def __call__(self, qkv, out):
+            return qkv[:, :512]
+    block = tp.TensorParallelBlockLinears(Backend(), 512, 256, 0, 1, _weights(tp, 512, 256, 1), 2, attention=Own())
+    x = np.random.default_rng(1).normal(size=(3, 512))
+    plain = tp.TensorParallelBlockLinears(Backend(), 512, 256, 0, 1, _weights(tp, 512, 256, 1), 2)
+    assert np.array_equal(block.forward(x), plain.forward(x))
+
+
 @pytest.mark.gpu
 def test_a_grouped_block_on_the_gpu(abq, cuda, tp):
     """A prompt and a token step through a block of 8 heads on 2: the attention gets its heads of the projection's rows; with queries and keys turned by a callable
